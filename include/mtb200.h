@@ -41,11 +41,13 @@ enum {
   MTB200_ERR_NOMEM = 3,        /* device allocation failed                               */
   MTB200_ERR_UNSUPPORTED = 4,  /* dtype / option not available for this operation        */
   MTB200_ERR_DEVICE_WAIT = 5,  /* a bounded wait inside a kernel ran out (see mtb200_sync) */
-  MTB200_ERR_BAD_LABEL = 6     /* class index outside [0, C) seen by cross entropy       */
+  MTB200_ERR_BAD_LABEL = 6     /* class index or token outside [0, C) seen by a loss      */
 };
 
 /* element types, numbered like minitensor's DataType (engine/src/tensor/dtype.rs:12-19) */
 enum { MTB200_F32 = 0, MTB200_F64 = 1, MTB200_I32 = 2, MTB200_I64 = 3, MTB200_BOOL = 4 };
+/* 16-bit types, which minitensor does not have: taken by the vocabulary operators only */
+enum { MTB200_F16 = 5, MTB200_BF16 = 6 };
 
 /* epilogues fused into mtb200_gemm */
 enum {
@@ -267,6 +269,54 @@ int32_t mtb200_adam_step(mtb200_handle h, int64_t n, float* param, const float* 
 int32_t mtb200_cross_entropy_ex(mtb200_handle h, int64_t B, int64_t C, const float* logits,
                                 const void* targets, int32_t target_dtype, int32_t reduction,
                                 float upstream, const float* upstream_rows, float* loss, float* dlogits);
+
+/* ---- vocabulary operators: log probabilities of given tokens, and distillation from top logits
+ * (No counterpart in the reference, whose classification losses end at cross_entropy_loss,
+ * engine/src/operations/loss/regression.rs:178-251; these are what a language model's head needs beside it.)
+ * logits: [rows][vocab], dtype MTB200_F32, MTB200_F16 or MTB200_BF16, row r at logits + r * ld elements (ld >= vocab: a
+ * vocabulary padded in memory; any alignment of the element type).  Sums and statistics are f32; a gradient is rounded
+ * once, to the logits' type.  temperature T > 0 divides the logits: z = x / T, p = softmax(z).
+ * Rows without a distribution: all logits -inf -> every log p is -inf, p and the entropy are 0; a NaN or +inf logit
+ * makes the row's results NaN.
+ * These calls use none of the handle's scratch memory, and are deterministic.
+ *
+ * token_log_probs: log_probs[r] = log p of tokens[r] (int32 / int64 [rows]; NULL: none, log_probs unused);
+ *   entropy[r] = -sum p log p (NULL: not wanted); the `top` (0 .. min(256, vocab)) largest logits of each row, best
+ *   first, ties to the lower index, NaN ranked with -inf: top_log_probs / top_indices [rows][top].
+ *   stats [rows][2] receives the row maximum and ln sum exp((x - max) / T), which the backward call reads.
+ *   With has_ignore, a row whose token equals ignore_index is left out: log probability and entropy 0, top entries
+ *   -inf with index -1, gradient 0, its logits are not read.  Another token outside [0, vocab) is reported by the next
+ *   mtb200_sync as MTB200_ERR_BAD_LABEL; its log probability is NaN.
+ * token_log_probs_bwd: dlogits (laid out with the same ld, must not overlap the logits) = the gradient of
+ *   sum d_log_probs * log_probs + d_entropy * entropy + d_top * top_log_probs; each of the three may be NULL (top = 0
+ *   for the last).  stats, entropy and top_indices are the forward call's; entries with index -1 are skipped. */
+int32_t mtb200_token_log_probs(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits,
+                               int64_t ld, const void* tokens, int32_t token_dtype, int32_t has_ignore,
+                               int64_t ignore_index, double temperature, int64_t top, float* log_probs,
+                               float* entropy, float* top_log_probs, int32_t* top_indices, float* stats);
+int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits,
+                                   int64_t ld, const void* tokens, int32_t token_dtype, int32_t has_ignore,
+                                   int64_t ignore_index, double temperature, const float* stats,
+                                   const float* d_log_probs, const float* entropy, const float* d_entropy,
+                                   int64_t top, const int32_t* top_indices, const float* d_top, void* dlogits);
+/* distill: Kullback-Leibler divergence of the student's p from a teacher known by `top` (0 .. 1024) entries per row,
+ *   teacher_indices [rows][top] (int32 / int64) and teacher_logits [rows][top] (f32 / f16 / bf16; logits or log
+ *   probabilities alike):  q = softmax(teacher_logits / T) over the entries whose index is not -1,
+ *   row_loss[r] = T^2 * sum_k q_k (log q_k - log p[teacher_indices_k]).
+ *   row_loss [rows] is always written; loss: one float for MTB200_REDUCE_SUM / MEAN (over all rows), unused for NONE.
+ *   dlogits (nullable, same ld) receives T * (sum q * p - q) * (MEAN ? 1/rows : 1) * upstream * (upstream_rows ?
+ *   upstream_rows[r] : 1).  stats (nullable, [rows][2]) as above.  A row without an entry (all -1, or all values -inf)
+ *   has loss 0 and gradient 0.  An index may come several times in a row: its weights add up.  Indices outside
+ *   [-1, vocab) are reported by the next mtb200_sync as MTB200_ERR_BAD_LABEL and treated as -1.
+ * distill_bwd: dlogits alone, from the stats of a forward call with the same logits and temperature. */
+int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                       int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                       int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                       const float* upstream_rows, float* row_loss, float* loss, float* stats, void* dlogits);
+int32_t mtb200_distill_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                           int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                           int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                           const float* upstream_rows, const float* stats, void* dlogits);
 
 /* ---- SGD step over one flat buffer (f32 / f64), in place
  * SGD::apply_simple_update / apply_momentum_update (engine/src/optim/sgd.rs:169-296):

@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmtb200.so")
 
 OK, ERR_INVALID, ERR_CUDA, ERR_NOMEM, ERR_UNSUPPORTED, ERR_DEVICE_WAIT, ERR_BAD_LABEL = range(7)
-F32, F64, I32, I64, BOOL = range(5)
+F32, F64, I32, I64, BOOL, F16, BF16 = range(7)
 EPI_NONE, EPI_RELU, EPI_GELU_ERF, EPI_GELU_TANH, EPI_RELU_BWD = range(5)
 
 _i32, _i64, _vp, _f32, _f64 = C.c_int32, C.c_int64, C.c_void_p, C.c_float, C.c_double
@@ -51,6 +51,14 @@ SIGNATURES = {
     "mtb200_bias_act": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp]),
     "mtb200_cross_entropy": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32, _vp, _vp]),
     "mtb200_cross_entropy_ex": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _vp]),
+    "mtb200_token_log_probs": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _f64, _i64, _vp, _vp, _vp, _vp,
+                                      _vp]),
+    "mtb200_token_log_probs_bwd": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _f64, _vp, _vp, _vp, _vp,
+                                          _i64, _vp, _vp, _vp]),
+    "mtb200_distill": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp, _vp,
+                              _vp, _vp]),
+    "mtb200_distill_bwd": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp,
+                                  _vp]),
     "mtb200_batch_norm_fwd": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _f64, _f64, _vp, _vp, _vp]),
     "mtb200_batch_norm_bwd": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "mtb200_dropout_mask": (_i32, [_vp, _i32, _i64, _f64, C.c_uint64, C.c_uint64, _vp]),

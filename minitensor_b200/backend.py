@@ -9,13 +9,13 @@ device memory and streams only); every computation goes through the C ABI.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (EPI_GELU_ERF, EPI_GELU_TANH, EPI_NONE, EPI_RELU, EPI_RELU_BWD, F32, F64, I32,
+from ._lib import (BF16, EPI_GELU_ERF, EPI_GELU_TANH, EPI_NONE, EPI_RELU, EPI_RELU_BWD, F16, F32, F64, I32,
                    I64, check)
 
 # the current stream's handle without building a torch.cuda.Stream object per call (a few microseconds on a path
@@ -23,6 +23,17 @@ from ._lib import (EPI_GELU_ERF, EPI_GELU_TANH, EPI_NONE, EPI_RELU, EPI_RELU_BWD
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 _DTYPES = {torch.float32: F32, torch.float64: F64, torch.int32: I32, torch.int64: I64}
+_LOGIT_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}  # the vocabulary operators' types
+_REDUCTIONS = {"sum": 0, "mean": 1, "none": 2}
+
+
+class TokenLogProbs(NamedTuple):
+    """Result of :meth:`Backend.token_log_probs`; outputs that were not asked for are ``None``."""
+    log_probs: Optional[torch.Tensor]       # [rows] float32
+    entropy: Optional[torch.Tensor]         # [rows] float32
+    top_log_probs: Optional[torch.Tensor]   # [rows, top] float32, best first
+    top_indices: Optional[torch.Tensor]     # [rows, top] int32
+    stats: torch.Tensor                     # [rows, 2] float32, for the backward call
 
 
 def dtype_code(t: torch.Tensor) -> int:
@@ -363,6 +374,157 @@ class Backend:
         self.launches += 1 if red == 2 else 2
         return loss, dl
 
+    # ------------------------------------------------------------------ vocabulary operators
+    def _on_device(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{what}: tensor on {t.device}, backend on {self.device}")
+
+    def _logit_rows(self, what: str, logits: torch.Tensor):
+        """(type code, rows, vocabulary, row stride) of a logit matrix; rows may be longer in memory than they are."""
+        code = _LOGIT_DTYPES.get(logits.dtype)
+        if code is None:
+            raise TypeError(f"{what}: unsupported dtype {logits.dtype}; logits are float32, float16 or bfloat16")
+        if logits.dim() != 2:
+            raise ValueError(f"{what}: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+        self._on_device(what, logits)
+        rows, vocab = logits.shape
+        if rows == 0 or vocab == 0:
+            return code, rows, vocab, vocab
+        ld = logits.stride(0) if rows > 1 else vocab
+        if (vocab > 1 and logits.stride(1) != 1) or ld < vocab:
+            raise ValueError(f"{what}: each row of the logits must be dense and rows must not overlap, got strides {logits.stride()}")
+        return code, rows, vocab, ld
+
+    def _vector(self, what: str, t: Optional[torch.Tensor], shape, dtypes) -> None:
+        if t is None:
+            return
+        if t.dtype not in dtypes:
+            raise TypeError(f"{what}: dtype {t.dtype} is not one of {', '.join(str(d) for d in dtypes)}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: shape mismatch: expected {list(shape)}, got {list(t.shape)}")
+        self._on_device(what, t)
+
+    @staticmethod
+    def _grad_like(logits: torch.Tensor, rows: int, vocab: int, ld: int) -> torch.Tensor:
+        """A gradient buffer with the logits' row stride and offset within 16 bytes, so that both move in whole vectors."""
+        off = (logits.data_ptr() & 15) // logits.element_size()
+        if (off == 0 and ld == vocab) or rows == 0:
+            return torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+        flat = torch.empty(off + (rows - 1) * ld + vocab, dtype=logits.dtype, device=logits.device)
+        return flat.as_strided((rows, vocab), (ld, 1), off)
+
+    def token_log_probs(self, logits: torch.Tensor, tokens: Optional[torch.Tensor], *, temperature: float = 1.0, top: int = 0,
+                        entropy: bool = False, ignore_index: Optional[int] = None) -> TokenLogProbs:
+        """Log probability of ``tokens[r]`` under ``softmax(logits[r] / temperature)``, the entropy of that distribution
+        and its ``top`` largest entries (best first, ties to the lower index), in one pass over ``logits``.
+
+        ``logits`` is ``[rows, vocabulary]`` in float32, float16 or bfloat16 with dense rows at any row stride;
+        ``tokens`` ``[rows]`` int32 / int64 or ``None``.  Rows whose token is ``ignore_index`` are left out: 0, 0, and
+        alternatives of -inf with index -1.  A token outside the vocabulary gives NaN and an ``IndexError`` at the next
+        :meth:`sync`."""
+        what = "token_log_probs"
+        code, rows, vocab, ld = self._logit_rows(what, logits)
+        self._vector(what, tokens, (rows,), (torch.int32, torch.int64))
+        if top < 0 or top > vocab:
+            raise ValueError(f"{what}: top must be between 0 and the vocabulary's {vocab} entries, got {top}")
+        dev, f32 = logits.device, torch.float32
+        out = TokenLogProbs(torch.empty(rows, dtype=f32, device=dev) if tokens is not None else None,
+                            torch.empty(rows, dtype=f32, device=dev) if entropy else None,
+                            torch.empty(rows, top, dtype=f32, device=dev) if top else None,
+                            torch.empty(rows, top, dtype=torch.int32, device=dev) if top else None,
+                            torch.empty(rows, 2, dtype=f32, device=dev))
+        self._bind_stream()
+        check(self.lib.mtb200_token_log_probs(
+            self._h, code, rows, vocab, logits.data_ptr(), ld, _ptr(tokens), I32 if tokens is None else _DTYPES[tokens.dtype],
+            ignore_index is not None, ignore_index or 0, temperature, top, _ptr(out.log_probs), _ptr(out.entropy),
+            _ptr(out.top_log_probs), _ptr(out.top_indices), _ptr(out.stats)))
+        self.launches += 1
+        return out
+
+    def token_log_probs_bwd(self, logits: torch.Tensor, tokens: Optional[torch.Tensor], stats: torch.Tensor, *,
+                            d_log_probs: Optional[torch.Tensor] = None, entropy: Optional[torch.Tensor] = None,
+                            d_entropy: Optional[torch.Tensor] = None, top_indices: Optional[torch.Tensor] = None,
+                            d_top: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                            ignore_index: Optional[int] = None) -> torch.Tensor:
+        """Gradient with respect to ``logits`` of :meth:`token_log_probs`, given the gradients of its outputs (any may be
+        ``None``) and what it returned; laid out in memory as the logits are, in their type."""
+        what = "token_log_probs_bwd"
+        code, rows, vocab, ld = self._logit_rows(what, logits)
+        self._vector(what, tokens, (rows,), (torch.int32, torch.int64))
+        f32 = (torch.float32,)
+        self._vector(what, stats, (rows, 2), f32)
+        for t in (d_log_probs, d_entropy, entropy if d_entropy is not None else None):
+            self._vector(what, t, (rows,), f32)
+        if (d_log_probs is not None and tokens is None) or (d_entropy is not None and entropy is None) or (
+                d_top is not None and top_indices is None):
+            raise ValueError(f"{what}: a gradient needs the tokens, the entropy or the indices that belong to it")
+        top = 0
+        if d_top is not None:
+            top = top_indices.shape[1] if top_indices.dim() == 2 else -1
+            self._vector(what, top_indices, (rows, top), (torch.int32,))
+            self._vector(what, d_top, (rows, top), f32)
+        grad = self._grad_like(logits, rows, vocab, ld)
+        self._bind_stream()
+        check(self.lib.mtb200_token_log_probs_bwd(
+            self._h, code, rows, vocab, logits.data_ptr(), ld, _ptr(tokens), I32 if tokens is None else _DTYPES[tokens.dtype],
+            ignore_index is not None, ignore_index or 0, temperature, _ptr(stats), _ptr(d_log_probs),
+            _ptr(entropy) if d_entropy is not None else None, _ptr(d_entropy), top, _ptr(top_indices) if top else None,
+            _ptr(d_top) if top else None, grad.data_ptr()))
+        self.launches += 1
+        return grad
+
+    def _distill_checks(self, what, logits, teacher_indices, teacher_logits, reduction, upstream_rows, stats):
+        code, rows, vocab, ld = self._logit_rows(what, logits)
+        red = _REDUCTIONS.get(reduction)
+        if red is None:
+            raise ValueError(f"Invalid reduction mode: {reduction}. Must be 'mean', 'sum', or 'none'")
+        if teacher_indices.dim() != 2:
+            raise ValueError(f"{what}: teacher indices must be [rows, entries], got {tuple(teacher_indices.shape)}")
+        top = teacher_indices.shape[1]
+        self._vector(what, teacher_indices, (rows, top), (torch.int32, torch.int64))
+        self._vector(what, teacher_logits, (rows, top), tuple(_LOGIT_DTYPES))
+        self._vector(what, upstream_rows, (rows,), (torch.float32,))
+        self._vector(what, stats, (rows, 2), (torch.float32,))
+        return code, rows, vocab, ld, red, top
+
+    def distillation_loss(self, logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor, *,
+                          temperature: float = 1.0, reduction: str = "mean", upstream: float = 1.0,
+                          upstream_rows: Optional[torch.Tensor] = None, want_grad: bool = True,
+                          stats: Optional[torch.Tensor] = None):
+        """``temperature**2 * KL(q || softmax(logits / temperature))`` per row, where ``q`` is the softmax of
+        ``teacher_logits / temperature`` over the teacher's entries ``[rows, entries]`` (logits or log probabilities;
+        index -1 marks a missing entry).  Returns ``(loss, dlogits or None)`` as :meth:`cross_entropy_ex` does; with
+        ``stats`` (``[rows, 2]`` float32) the statistics for :meth:`distillation_loss_bwd` are kept there."""
+        code, rows, vocab, ld, red, top = self._distill_checks("distillation_loss", logits, teacher_indices, teacher_logits,
+                                                               reduction, upstream_rows, stats)
+        row_loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        loss = row_loss if red == 2 else torch.empty(1, dtype=torch.float32, device=logits.device)
+        grad = self._grad_like(logits, rows, vocab, ld) if want_grad else None
+        self._bind_stream()
+        check(self.lib.mtb200_distill(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
+                                      _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
+                                      _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream, _ptr(upstream_rows),
+                                      _ptr(row_loss), None if red == 2 else _ptr(loss), _ptr(stats),
+                                      grad.data_ptr() if want_grad and grad.numel() else None))
+        self.launches += 1 if red == 2 else 2
+        return loss, grad
+
+    def distillation_loss_bwd(self, logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor,
+                              stats: torch.Tensor, *, temperature: float = 1.0, reduction: str = "mean", upstream: float = 1.0,
+                              upstream_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The gradient of :meth:`distillation_loss` alone, from the ``stats`` that it kept."""
+        code, rows, vocab, ld, red, top = self._distill_checks("distillation_loss_bwd", logits, teacher_indices, teacher_logits,
+                                                               reduction, upstream_rows, stats)
+        grad = self._grad_like(logits, rows, vocab, ld)
+        self._bind_stream()
+        check(self.lib.mtb200_distill_bwd(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
+                                          _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
+                                          _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream, _ptr(upstream_rows),
+                                          _ptr(stats), grad.data_ptr()))
+        self.launches += 1
+        return grad
+
     def sgd_step(self, p: torch.Tensor, g: torch.Tensor, v: Optional[torch.Tensor] = None, *, lr: float,
                  momentum: float = 0.0, dampening: float = 0.0, weight_decay: float = 0.0,
                  nesterov: bool = False) -> None:
@@ -547,5 +709,5 @@ def get_backend(device: int = 0) -> Backend:
     return _default[device]
 
 
-__all__ = ["Backend", "get_backend", "EPI_NONE", "EPI_RELU", "EPI_GELU_ERF", "EPI_GELU_TANH",
+__all__ = ["Backend", "TokenLogProbs", "get_backend", "EPI_NONE", "EPI_RELU", "EPI_GELU_ERF", "EPI_GELU_TANH",
            "EPI_RELU_BWD"]

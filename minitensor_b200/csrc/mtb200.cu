@@ -309,7 +309,7 @@ int32_t mtb200_sync(mtb200_handle h) {
       return fail(MTB200_ERR_DEVICE_WAIT,
                   "a bounded wait inside a GEMM kernel ran out (role %u, site %u); results are invalid",
                   wait_code >> 8, wait_code & 0xffu);
-    return fail(MTB200_ERR_BAD_LABEL, "cross entropy saw a class index outside [0, C)");
+    return fail(MTB200_ERR_BAD_LABEL, "a loss saw a class index or token outside [0, C)");
   }
   return MTB200_OK;
 }

@@ -16,7 +16,7 @@ the backward products are launched without materialised transposes.
 from __future__ import annotations
 
 import math
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -462,3 +462,112 @@ class CrossEntropyLoss(Module):
 
     def __call__(self, input: Tensor, target: Tensor) -> Tensor:
         return cross_entropy(input, target, self.reduction)
+
+
+class TokenLogProbs(NamedTuple):
+    """Result of :func:`token_log_probs`; outputs that were not asked for are ``None``."""
+    log_probs: Tensor
+    entropy: Optional[Tensor]
+    top_log_probs: Optional[Tensor]
+    top_indices: Optional[Tensor]
+
+
+def token_log_probs(input: Tensor, tokens: Tensor, temperature: float = 1.0, top: int = 0, entropy: bool = False,
+                    ignore_index: Optional[int] = None) -> TokenLogProbs:
+    """Log probability of one given token per position under ``softmax(input / temperature)``, with the entropy of that
+    distribution and its ``top`` most likely tokens on request (no counterpart in the reference).
+
+    ``input`` holds float32 logits ``[..., vocabulary]``, ``tokens`` int32 / int64 indices ``[...]``.  Positions whose
+    token is ``ignore_index`` are left out: 0, 0, alternatives of -inf with index -1, no gradient.  ``log_probs``,
+    ``entropy`` and ``top_log_probs`` are differentiable; one backward pass over the logits serves all of them."""
+    if input.ndim < 1:
+        raise ValueError("token_log_probs expects at least 1-D logits")
+    if input.dtype != "float32":
+        raise TypeError("token_log_probs on this path takes float32 logits")
+    if tokens.dtype not in ("int32", "int64"):
+        raise TypeError("tokens must be int32 or int64 indices")
+    lead, vocab = input.shape[:-1], input.shape[-1]
+    if tokens.shape != lead:
+        raise ValueError(f"shape mismatch: {input.shape} vs {tokens.shape}")
+    rows = tokens._buf.numel()
+    x2, t2 = input._buf.reshape(rows, vocab).contiguous(), tokens._buf.reshape(rows).contiguous()
+    be = _be()
+    res = be.token_log_probs(x2, t2, temperature=temperature, top=top, entropy=entropy, ignore_index=ignore_index)
+    be.sync()  # surfaces a token outside the vocabulary as IndexError, as cross_entropy does
+    # The outputs share one tape node, whose gradient holds theirs side by side: log probabilities, entropy, top.
+    width = 2 + top
+    used = set()
+
+    def bw(g):
+        want = set(used)
+        used.clear()
+        return (be.token_log_probs_bwd(
+            x2, t2, res.stats, d_log_probs=g[0] if "log_probs" in want else None, entropy=res.entropy,
+            d_entropy=g[1] if "entropy" in want else None, top_indices=res.top_indices,
+            d_top=g[2:].reshape(rows, top) if "top" in want else None, temperature=temperature,
+            ignore_index=ignore_index).reshape(input.shape),)
+
+    hub = input._result(res.stats, (input,), bw)
+
+    def output(name, buf, shape, first, count):
+        def spread(g):
+            used.add(name)
+            whole = torch.zeros(width, rows, dtype=torch.float32, device=buf.device)
+            whole[first:first + count] = g.reshape(count, rows)
+            return (whole,)
+        return hub._result(buf.reshape(shape), (hub,), spread)
+
+    return TokenLogProbs(
+        output("log_probs", res.log_probs, lead, 0, 1),
+        output("entropy", res.entropy, lead, 1, 1) if entropy else None,
+        output("top", res.top_log_probs, lead + (top,), 2, top) if top else None,
+        Tensor(None, _buf=res.top_indices.reshape(lead + (top,))) if top else None)
+
+
+def distillation_loss(input: Tensor, teacher_indices: Tensor, teacher_logits: Tensor, temperature: float = 1.0,
+                      reduction: str = "mean") -> Tensor:
+    """``temperature**2 * KL(q || softmax(input / temperature))`` where the teacher is known by its largest logits alone:
+    ``q = softmax(teacher_logits / temperature)`` over the entries ``teacher_indices`` ``[..., entries]`` of each position,
+    index -1 marking a missing one (no counterpart in the reference).
+
+    ``teacher_logits`` may be logits or log probabilities, e.g. the ``top_log_probs`` of :func:`token_log_probs` with its
+    ``top_indices``; no gradient flows to them.  ``input`` holds float32 logits ``[..., vocabulary]``.  A position without
+    an entry has loss 0 and gradient 0; ``reduction`` "mean" divides by the number of positions."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"Invalid reduction mode: {reduction}. Must be 'mean', 'sum', or 'none'")
+    if input.ndim < 1 or teacher_indices.ndim != input.ndim:
+        raise ValueError(f"shape mismatch: {input.shape} vs {teacher_indices.shape}")
+    if input.dtype != "float32" or teacher_logits.dtype != "float32":
+        raise TypeError("distillation_loss on this path takes float32 logits")
+    if teacher_indices.dtype not in ("int32", "int64"):
+        raise TypeError("teacher indices must be int32 or int64")
+    lead, vocab, top = input.shape[:-1], input.shape[-1], teacher_indices.shape[-1]
+    if teacher_indices.shape[:-1] != lead or teacher_logits.shape != teacher_indices.shape:
+        raise ValueError(f"shape mismatch: {input.shape}, {teacher_indices.shape}, {teacher_logits.shape}")
+    rows = 1
+    for d in lead:
+        rows *= d
+    x2 = input._buf.reshape(rows, vocab).contiguous()
+    idx = teacher_indices._buf.reshape(rows, top).contiguous()
+    val = teacher_logits._buf.reshape(rows, top).contiguous()
+    be = _be()
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x2.device) if input.requires_grad else None
+    loss, _ = be.distillation_loss(x2, idx, val, temperature=temperature, reduction=reduction, want_grad=False, stats=stats)
+    be.sync()  # surfaces an index outside the vocabulary as IndexError, as cross_entropy does
+
+    def bw(g):
+        up = g.reshape(rows) if reduction == "none" else g.reshape(1).expand(rows)
+        return (be.distillation_loss_bwd(x2, idx, val, stats, temperature=temperature, reduction=reduction,
+                                         upstream_rows=up.contiguous()).reshape(input.shape),)
+
+    return input._result(loss.reshape(lead) if reduction == "none" else loss.reshape(()), (input,), bw)
+
+
+class DistillationLoss(Module):
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError(f"Invalid reduction mode: {reduction}. Must be 'mean', 'sum', or 'none'")
+        self.temperature, self.reduction = temperature, reduction
+
+    def __call__(self, input: Tensor, teacher_indices: Tensor, teacher_logits: Tensor) -> Tensor:
+        return distillation_loss(input, teacher_indices, teacher_logits, self.temperature, self.reduction)
