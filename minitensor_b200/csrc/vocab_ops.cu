@@ -41,20 +41,78 @@ struct ScoreArgs {
   uint32_t* bad_label;
 };
 
+constexpr int MAX_PARTS = 8;  // blocks of a portable cluster
+
+// A block works on one part of one row, or, where rows are short, each of its warps on a row of its own.
+template <int G>
+struct Block {
+  static constexpr int ROWS = G == 32 ? 8 : 1;
+  static constexpr int THREADS = G * ROWS;
+  static __device__ __forceinline__ int slot() { return G == 32 ? threadIdx.x >> 5 : 0; }
+  // row index, or -1 behind the last one (then the whole group has nothing to do)
+  static __device__ __forceinline__ long long row(int rows, int parts) {
+    const long long r = G == 32 ? static_cast<long long>(blockIdx.x) * ROWS + slot() : blockIdx.x / parts;
+    return r < rows ? r : -1;
+  }
+  static __device__ __forceinline__ int part(int parts) { return G == 32 ? 0 : blockIdx.x % parts; }
+};
+
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.442695040888963407f;
 
 // ------------------------------------------------------------------ token log probabilities
-// A cluster of `parts` blocks per row (one block when there are rows enough).  One pass over the logits: HBM-bound.
-template <typename T, int THREADS, bool TOP, bool ENT>
-static __global__ void __launch_bounds__(THREADS) token_scores_kernel(ScoreArgs a) {
+template <bool TOP, bool ENT>
+__device__ __forceinline__ void put_left_out(const ScoreArgs& a, long long r, int tid, int threads) {
+  if (tid == 0) {
+    a.log_probs[r] = 0.0f;
+    if (ENT) a.entropy[r] = 0.0f;
+    a.stats[2 * r] = -INFINITY;
+    a.stats[2 * r + 1] = 0.0f;
+  }
+  if (TOP)
+    for (int i = tid; i < a.top; i += threads) {
+      a.top_log_probs[r * a.top + i] = -INFINITY;
+      a.top_indices[r * a.top + i] = -1;
+    }
+}
+// A row's results from its statistics.
+template <bool ENT>
+struct RowOut {
+  long long r;
+  RowStat st;
+  bool none;  // no distribution
+  float ln_s;
+  __device__ __forceinline__ RowOut(const ScoreArgs& a, long long row, const RowStat& stat) : r(row), st(stat) {
+    none = st.m == -INFINITY && !isnan(st.s);
+    ln_s = none ? 0.0f : logf(st.s);
+  }
+  __device__ __forceinline__ void put_scores(const ScoreArgs& a, float x_token, bool good) const {
+    if (a.log_probs) a.log_probs[r] = none && good ? -INFINITY : (x_token - st.m) * a.inv_t - ln_s;
+    if (ENT) a.entropy[r] = none ? 0.0f : ln_s - a.inv_t * (st.u / st.s);
+    a.stats[2 * r] = st.m;
+    a.stats[2 * r + 1] = ln_s;
+  }
+  __device__ __forceinline__ void put_top(const ScoreArgs& a, int at, unsigned long long w) const {
+    a.top_log_probs[r * a.top + at] = none ? -INFINITY : (key_value(candidate_key(w)) - st.m) * a.inv_t - ln_s;
+    a.top_indices[r * a.top + at] = candidate_index(w);
+  }
+};
+
+// A cluster of `parts` blocks per row (one block when there are rows enough, a warp for short rows).  One pass over the
+// logits: HBM-bound.  Registers decide how many blocks share an SM: three of 512 threads without the selection; with it
+// 1024 threads, whose 64 registers keep the four loads of a round together.
+template <typename T, int G, bool TOP, bool ENT>
+static __global__ void __launch_bounds__(Block<G>::THREADS, TOP ? (G >= 256 ? 1024 / G : 1) : (G == 512 ? 3 : 1)) token_scores_kernel(ScoreArgs a) {
   using L = LogitType<T>;
-  __shared__ RowStat sm[THREADS / 32 + 1];
-  __shared__ TopScratch<TOP ? THREADS : 32> ts;
+  extern __shared__ __align__(16) unsigned char dynamic_smem[];
+  __shared__ RowStat sm[Group<G>::WARPS + 1], parts_st[MAX_PARTS];
+  TopScratch<G>& ts = reinterpret_cast<TopScratch<G>*>(dynamic_smem)[Block<G>::slot()];  // with TOP
+  unsigned long long* lists = reinterpret_cast<unsigned long long*>(dynamic_smem + sizeof(TopScratch<G>));  // [parts][top]
   cg::cluster_group cluster = cg::this_cluster();
-  const int part = blockIdx.x % a.parts;
-  const long long r = blockIdx.x / a.parts;
-  const int tid = threadIdx.x;
+  const int part = Block<G>::part(a.parts);
+  const long long r = Block<G>::row(a.rows, a.parts);
+  const int tid = Group<G>::rank();
+  if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
 
   long long token = -1;
@@ -62,71 +120,53 @@ static __global__ void __launch_bounds__(THREADS) token_scores_kernel(ScoreArgs 
   if (a.tokens.p) {
     token = a.tokens.at(r);
     if (a.has_ignore && token == a.ignore) {  // the whole cluster leaves
-      if (part == 0) {
-        if (tid == 0) {
-          a.log_probs[r] = 0.0f;
-          if (ENT) a.entropy[r] = 0.0f;
-          a.stats[2 * r] = -INFINITY;
-          a.stats[2 * r + 1] = 0.0f;
-        }
-        if (TOP)
-          for (int i = tid; i < a.top; i += THREADS) {
-            a.top_log_probs[r * a.top + i] = -INFINITY;
-            a.top_indices[r * a.top + i] = -1;
-          }
-      }
+      if (part == 0) put_left_out<TOP, ENT>(a, r, tid, G);
       return;
     }
     good = token >= 0 && token < a.vocab;
     if (!good && part == 0 && tid == 0) atomicOr(a.bad_label, 1u);
   }
+  const bool split = G > 32 && a.parts > 1;
+  if (split) cluster.barrier_arrive();  // waited for before the first block's memory is written to
   float x_token = 0.0f;
   if (part == 0 && tid == 0 && a.tokens.p) x_token = good ? L::up(row[token]) : NAN;
 
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
-  int where;
-  const RowStat unit = unit_stats<T, THREADS, ENT>(p, a.c, where);
-  RowStat st = block_merge<THREADS>(unit, a.c, sm);
-  if constexpr (TOP) select_top<T, THREADS>(p, a.top, unit.m, where, ts);
-  if (a.parts > 1) {
+  const UnitStat unit = unit_stats<T, G, ENT, TOP>(p, a.c, ts.slots);
+  RowStat st = group_merge<G>(unit.sum(), a.c, sm);
+  if constexpr (TOP) select_top<T, G>(p, a.top, unit.m, unit.where, ts);
+  if (split) {
+    cluster.barrier_wait();
+    if (tid == 0) *cluster.map_shared_rank(&parts_st[part], 0) = st;
+    if constexpr (TOP)
+      for (int i = tid; i < a.top; i += G) cluster.map_shared_rank(lists, 0)[part * a.top + i] = ts.best[i];
     cluster.sync();
-    if (part == 0) st = cluster_merge(cluster, &sm[THREADS / 32], a.parts, a.c);
+    if (part) return;
+    st = parts_merge(parts_st, a.parts, a.c);
   }
-  if (part == 0) {
-    const bool none = st.m == -INFINITY && !isnan(st.s);
-    const float ln_s = none ? 0.0f : logf(st.s);
-    if (tid == 0) {
-      if (a.log_probs) a.log_probs[r] = none && good ? -INFINITY : (x_token - st.m) * a.inv_t - ln_s;
-      if (ENT) a.entropy[r] = none ? 0.0f : ln_s - a.inv_t * (st.u / st.s);
-      a.stats[2 * r] = st.m;
-      a.stats[2 * r + 1] = ln_s;
-    }
-    if constexpr (TOP) {
-      auto put = [&](int at, unsigned long long w) {
-        a.top_log_probs[r * a.top + at] = none ? -INFINITY : (key_value(candidate_key(w)) - st.m) * a.inv_t - ln_s;
-        a.top_indices[r * a.top + at] = candidate_index(w);
-      };
-      if (a.parts == 1) {
-        for (int i = tid; i < a.top; i += THREADS) put(i, ts.best[i]);
-      } else {
-        // merge of the parts' sorted lists: an entry's place is its place in its own list plus the entries above it
-        // in every other one
-        unsigned long long* pool = ts.pool;  // parts * top <= 8 * 256 words
-        const int total = a.parts * a.top;
-        for (int i = tid; i < total; i += THREADS) pool[i] = cluster.map_shared_rank(ts.best, i / a.top)[i % a.top];
-        __syncthreads();
-        for (int i = tid; i < total; i += THREADS) {
-          const unsigned long long w = pool[i];
-          if (!w) continue;
-          int at = i % a.top;
-          for (int q = 0; q < a.parts && at < a.top; ++q)
-            if (q != i / a.top) at += count_above(pool + q * a.top, a.top, w);
-          if (at < a.top) put(at, w);
-        }
+  const RowOut<ENT> out(a, r, st);
+  if (tid == 0) out.put_scores(a, x_token, good);
+  if constexpr (TOP) {
+    if (!split) {
+      for (int i = tid; i < a.top; i += G) out.put_top(a, i, ts.best[i]);
+    } else {
+      // The parts' sorted lists together hold at least `top` entries at or above the least of their
+      // ceil(top / parts)-th ones; those that reach it are counted against each other.
+      const int nth = (a.top + a.parts - 1) / a.parts - 1;
+      unsigned long long bound = ~0ull;
+      for (int q = 0; q < a.parts; ++q) bound = min(bound, lists[q * a.top + nth]);
+      if (tid == 0) ts.pool_count = 0;
+      Group<G>::sync();
+      for (int i = tid; i < a.parts * a.top; i += G) {  // at most 8 * 256 words
+        const unsigned long long w = lists[i];
+        if (w && w >= bound) ts.pool[atomicAdd(&ts.pool_count, 1)] = w;
       }
+      Group<G>::sync();
+      for_each_rank<G>(ts.pool, ts.pool_count, [&](int i, int above) {
+        if (above < a.top) out.put_top(a, above, ts.pool[i]);
+      });
     }
   }
-  if (a.parts > 1) cluster.sync();  // shared memory stays until rank 0 has read it
 }
 
 struct ScoreGradArgs {
@@ -144,27 +184,30 @@ struct ScoreGradArgs {
 };
 
 // dx = (1/T) [ sum of weights at given indices - p (sum of all weights) - g_H p (log p + H) ], one read, one write.
-template <typename T, int THREADS, bool ENT>
-static __global__ void __launch_bounds__(THREADS) token_scores_grad_kernel(ScoreGradArgs a) {
-  __shared__ int idx[VOCAB_TOP_MAX + 1];
-  __shared__ float weight[VOCAB_TOP_MAX + 1];
-  __shared__ float fold[THREADS / 32];
-  const int part = blockIdx.x % a.parts;
-  const long long r = blockIdx.x / a.parts;
-  const int tid = threadIdx.x;
+template <typename T, int G, bool ENT>
+static __global__ void __launch_bounds__(Block<G>::THREADS) token_scores_grad_kernel(ScoreGradArgs a) {
+  __shared__ int all_idx[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
+  __shared__ float all_weight[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
+  __shared__ float fold[Group<G>::WARPS];
+  int* idx = all_idx[Block<G>::slot()];
+  float* weight = all_weight[Block<G>::slot()];
+  const int part = Block<G>::part(a.parts);
+  const long long r = Block<G>::row(a.rows, a.parts);
+  const int tid = Group<G>::rank();
+  if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
   const long long token = a.tokens.p ? a.tokens.at(r) : -1;
   if (a.tokens.p && a.has_ignore && token == a.ignore) {
-    zero_grad<T, THREADS>(p, dx, a.same_phase);
+    zero_grad<T, G>(p, dx, a.same_phase);
     return;
   }
   const bool good = token >= 0 && token < a.vocab;
   if (a.tokens.p && !good && part == 0 && tid == 0) atomicOr(a.bad_label, 1u);
   const int n = a.top + 1;
   float sum = 0.0f;
-  for (int e = tid; e < n; e += THREADS) {
+  for (int e = tid; e < n; e += G) {
     int j;
     float w;
     if (e == 0) {
@@ -182,7 +225,7 @@ static __global__ void __launch_bounds__(THREADS) token_scores_grad_kernel(Score
     weight[e] = w * a.inv_t;
     sum += w;
   }
-  sum = block_fold<THREADS, false>(sum, fold);
+  sum = group_fold<G, false>(sum, fold);
   RowGrad g;
   const float m = a.stats[2 * r];
   g.base = m == -INFINITY ? 0.0f : m;
@@ -190,9 +233,9 @@ static __global__ void __launch_bounds__(THREADS) token_scores_grad_kernel(Score
   const float gh = ENT ? a.d_entropy[r] : 0.0f;
   g.b = -gh * a.inv_t * LN2;
   g.a = -a.inv_t * (sum + (ENT ? gh * a.entropy[r] : 0.0f));
-  dense_grad<T, THREADS, ENT>(p, dx, a.c, g, a.same_phase);
-  __syncthreads();
-  sparse_fix<T, THREADS, ENT>(p, dx, a.c, g, idx, weight, n);
+  dense_grad<T, G, ENT>(p, dx, a.c, g, a.same_phase);
+  Group<G>::sync();
+  sparse_fix<T, G, ENT>(p, dx, a.c, g, idx, weight, n);
 }
 
 // ------------------------------------------------------------------ distillation
@@ -210,16 +253,20 @@ struct DistillArgs {
   uint32_t* bad_label;
 };
 
+constexpr int TEACHER_WARP_MAX = 128;  // entries where a warp has a row of its own: 12 KB a block
+template <int G>
+constexpr int TEACHER_ROOM = G == 32 ? TEACHER_WARP_MAX : VOCAB_TEACHER_MAX;
+
 // The teacher's entries of row r into shared memory: q over the entries with an index in [0, vocab) (0 elsewhere,
 // index -1), softmax of value / T, and (nullable) dv = value - largest value.  Returns whether the row has any entry;
 // ln_s: log q = dv / T - ln_s (NaN if a value is NaN or +inf).
-template <int THREADS>
+template <int G>
 __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, bool report, int* idx, float* q, float* dv,
                                              float* fold, float* ln_s) {
-  const int tid = threadIdx.x;
+  const int tid = Group<G>::rank();
   float top = -INFINITY;
   bool any = false;
-  for (int e = tid; e < a.top; e += THREADS) {
+  for (int e = tid; e < a.top; e += G) {
     const long long j = a.index.at(r * a.top + e);
     const bool in = j >= 0 && j < a.vocab;
     if (!in && j != -1 && report) atomicOr(a.bad_label, 1u);
@@ -228,45 +275,48 @@ __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, 
     top = fmaxf(top, q[e]);
     any = any || (in && q[e] != -INFINITY);  // NaN counts: it has to reach the result
   }
-  any = __syncthreads_or(any);
+  any = G == 32 ? __any_sync(0xffffffffu, any) : Group<G>::count(any) > 0;
   if (!any) return false;
-  top = block_fold<THREADS, true>(top, fold);
+  top = group_fold<G, true>(top, fold);
   const float base = top == -INFINITY ? 0.0f : top;
   float s = 0.0f;
-  for (int e = tid; e < a.top; e += THREADS) {
+  for (int e = tid; e < a.top; e += G) {
     const float d = q[e] - base;
     const float w = ex2_ftz(d * a.c);
     s += w;
     q[e] = w;
     if (dv) dv[e] = d;
   }
-  s = block_fold<THREADS, false>(s, fold);
+  s = group_fold<G, false>(s, fold);
   const float inv = 1.0f / s;
-  for (int e = tid; e < a.top; e += THREADS) q[e] *= inv;
+  for (int e = tid; e < a.top; e += G) q[e] *= inv;
   *ln_s = logf(s);
-  __syncthreads();
+  Group<G>::sync();
   return true;
 }
 
 // Loss per row, T^2 sum_k q_k (log q_k - log p_idx_k), and with GRAD the gradient: the row's statistics, then a second
 // look at the row while it is in L2.
-template <typename T, int THREADS, bool GRAD>
-static __global__ void __launch_bounds__(THREADS) distill_kernel(DistillArgs a) {
+template <typename T, int G, bool GRAD>
+static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(DistillArgs a) {
   using L = LogitType<T>;
-  __shared__ RowStat sm[THREADS / 32 + 1];
-  __shared__ int idx[VOCAB_TEACHER_MAX];
-  __shared__ float q[VOCAB_TEACHER_MAX], dv[VOCAB_TEACHER_MAX];
-  __shared__ float fold[THREADS / 32];
+  __shared__ RowStat sm[Group<G>::WARPS + 1], parts_st[MAX_PARTS];
+  __shared__ int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>], all_dv[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ float fold[Group<G>::WARPS];
+  int* idx = all_idx[Block<G>::slot()];
+  float *q = all_q[Block<G>::slot()], *dv = all_dv[Block<G>::slot()];
   cg::cluster_group cluster = cg::this_cluster();
-  const int part = blockIdx.x % a.parts;
-  const long long r = blockIdx.x / a.parts;
-  const int tid = threadIdx.x;
+  const int part = Block<G>::part(a.parts);
+  const long long r = Block<G>::row(a.rows, a.parts);
+  const int tid = Group<G>::rank();
+  if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   T* dx = GRAD ? static_cast<T*>(a.dlogits) + r * a.ld : nullptr;
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
 
   float ln_sq;
-  if (!load_teacher<THREADS>(a, r, part == 0, idx, q, dv, fold, &ln_sq)) {  // the same answer in every block of the cluster
+  if (!load_teacher<G>(a, r, part == 0, idx, q, dv, fold, &ln_sq)) {  // the same answer in every block of the cluster
     if (part == 0 && tid == 0) {
       a.row_loss[r] = 0.0f;
       if (a.stats) {
@@ -274,26 +324,29 @@ static __global__ void __launch_bounds__(THREADS) distill_kernel(DistillArgs a) 
         a.stats[2 * r + 1] = 0.0f;
       }
     }
-    if (GRAD) zero_grad<T, THREADS>(p, dx, a.same_phase);
+    if (GRAD) zero_grad<T, G>(p, dx, a.same_phase);
     return;
   }
-  int where;
-  RowStat st = block_merge<THREADS>(unit_stats<T, THREADS, false>(p, a.c, where), a.c, sm);
-  if (a.parts > 1) {
+  const bool split = G > 32 && a.parts > 1;
+  if (split) cluster.barrier_arrive();  // waited for before another block's memory is written to
+  RowStat st = group_merge<G>(unit_stats<T, G, false, false>(p, a.c, nullptr).sum(), a.c, sm);
+  if (split) {
+    cluster.barrier_wait();
+    if (tid < a.parts) *cluster.map_shared_rank(&parts_st[part], tid) = st;
     cluster.sync();
-    st = cluster_merge(cluster, &sm[THREADS / 32], a.parts, a.c);
+    st = parts_merge(parts_st, a.parts, a.c);
   }
   const bool none = st.m == -INFINITY && !isnan(st.s);
   const float ln_s = none ? 0.0f : logf(st.s);
   if (part == 0) {
     // log q - log p with the two maxima taken out first: nearly equal distributions lose nothing to the logarithms' size
     float kl = 0.0f;
-    for (int e = tid; e < a.top; e += THREADS) {
+    for (int e = tid; e < a.top; e += G) {
       if (idx[e] < 0 || q[e] == 0.0f) continue;
       const float dx = none ? -INFINITY : L::up(row[idx[e]]) - st.m;
       kl += q[e] * ((dv[e] - dx) * a.inv_t - (ln_sq - ln_s));
     }
-    kl = block_fold<THREADS, false>(kl, fold);
+    kl = group_fold<G, false>(kl, fold);
     if (tid == 0) {
       a.row_loss[r] = a.t * a.t * kl;
       if (a.stats) {
@@ -309,27 +362,29 @@ static __global__ void __launch_bounds__(THREADS) distill_kernel(DistillArgs a) 
     const float scale = a.upstream_rows ? a.scale * a.upstream_rows[r] : a.scale;
     g.a = isnan(ln_sq) ? NAN : scale;
     g.b = 0.0f;
-    dense_grad<T, THREADS, false>(p, dx, a.c, g, a.same_phase);
-    for (int e = tid; e < a.top; e += THREADS) q[e] *= -scale;
-    __syncthreads();
-    sparse_fix<T, THREADS, false>(p, dx, a.c, g, idx, q, a.top);
+    dense_grad<T, G, false>(p, dx, a.c, g, a.same_phase);
+    for (int e = tid; e < a.top; e += G) q[e] *= -scale;
+    Group<G>::sync();
+    sparse_fix<T, G, false>(p, dx, a.c, g, idx, q, a.top);
   }
-  if (a.parts > 1) cluster.sync();
 }
 
-template <typename T, int THREADS>
-static __global__ void __launch_bounds__(THREADS) distill_grad_kernel(DistillArgs a) {
-  __shared__ int idx[VOCAB_TEACHER_MAX];
-  __shared__ float q[VOCAB_TEACHER_MAX];
-  __shared__ float fold[THREADS / 32];
-  const int part = blockIdx.x % a.parts;
-  const long long r = blockIdx.x / a.parts;
+template <typename T, int G>
+static __global__ void __launch_bounds__(Block<G>::THREADS) distill_grad_kernel(DistillArgs a) {
+  __shared__ int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ float fold[Group<G>::WARPS];
+  int* idx = all_idx[Block<G>::slot()];
+  float* q = all_q[Block<G>::slot()];
+  const int part = Block<G>::part(a.parts);
+  const long long r = Block<G>::row(a.rows, a.parts);
+  if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
   float ln_sq;
-  if (!load_teacher<THREADS>(a, r, part == 0, idx, q, nullptr, fold, &ln_sq)) {
-    zero_grad<T, THREADS>(p, dx, a.same_phase);
+  if (!load_teacher<G>(a, r, part == 0, idx, q, nullptr, fold, &ln_sq)) {
+    zero_grad<T, G>(p, dx, a.same_phase);
     return;
   }
   RowGrad g;
@@ -339,10 +394,10 @@ static __global__ void __launch_bounds__(THREADS) distill_grad_kernel(DistillArg
   const float scale = a.upstream_rows ? a.scale * a.upstream_rows[r] : a.scale;
   g.a = isnan(ln_sq) ? NAN : scale;
   g.b = 0.0f;
-  dense_grad<T, THREADS, false>(p, dx, a.c, g, a.same_phase);
-  for (int e = threadIdx.x; e < a.top; e += THREADS) q[e] *= -scale;
-  __syncthreads();
-  sparse_fix<T, THREADS, false>(p, dx, a.c, g, idx, q, a.top);
+  dense_grad<T, G, false>(p, dx, a.c, g, a.same_phase);
+  for (int e = Group<G>::rank(); e < a.top; e += G) q[e] *= -scale;
+  Group<G>::sync();
+  sparse_fix<T, G, false>(p, dx, a.c, g, idx, q, a.top);
 }
 
 // Sum or mean of the row losses, in f64 and a fixed order.
@@ -389,54 +444,82 @@ static int32_t check_index(const char* what, int32_t dtype) {
   return MTB200_OK;
 }
 
-// Launch of one cluster of `parts` blocks per row.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_rows(mtb200_ctx* h, void (*kernel)(KArgs...), int64_t rows, int parts, int threads, Args... args) {
+// One cluster of `parts` blocks per row, or with G = 32 a warp per row.  Kernels whose blocks do not meet take a plain
+// grid (`meet` false).
+template <int G, typename Args>
+static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, bool meet, size_t smem = 0) {
+  if (smem > 48 * 1024)
+    if (int32_t rc = grant_dynamic_smem(h, kernel, int(smem))) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows * parts));
-  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(G == 32 ? unsigned((a.rows + Block<G>::ROWS - 1) / Block<G>::ROWS) : unsigned(a.rows) * unsigned(a.parts));
+  cfg.blockDim = dim3(unsigned(Block<G>::THREADS));
   cfg.stream = h->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(parts);
+  attr[0].val.clusterDim.x = unsigned(a.parts);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  cfg.numAttrs = meet && a.parts > 1 ? 1 : 0;
+  MTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  return MTB200_OK;
 }
 
-// Blocks per row: one when the rows fill the machine, else up to 8 with at least `least` bytes of the row each.
-static int row_parts(const mtb200_ctx* h, int64_t rows, int64_t row_bytes) {
+// Threads per row and blocks per row.
+struct RowPlan {
+  int group, parts;
+};
+// A warp per row up to 8 KB (65536 x 1000 f32: 57 us against 460 us with a block of 512 per row), 128 threads up to 32 KB,
+// else blocks of 512.  Where whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long
+// as the parts still find room side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us
+// in 8, which run in two waves.
+constexpr int64_t WARP_BYTES = 8192, MID_BYTES = 32768, PART_BYTES = 8192;
+static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, int64_t warp_top, int64_t mid_top, int64_t top) {
+  if (row_bytes <= WARP_BYTES && top <= warp_top && rows > h->sm_count) return {32, 1};
+  if (row_bytes <= MID_BYTES && top <= mid_top) return {128, 1};
   int parts = 1;
-  while (parts < 8 && rows * parts < 2 * h->sm_count && row_bytes / (2 * parts) >= 8192) parts *= 2;
-  return parts;
+  while (parts < MAX_PARTS && rows * parts <= h->sm_count && row_bytes / (2 * parts) >= PART_BYTES) parts *= 2;
+  return {512, parts};
 }
 
-template <typename T, int THREADS>
+// With the selection on rows of 16-bit logits, four blocks of 256 threads on an SM instead of two of 512: a block that selects
+// leaves three that stream.  4096 x 128256 bf16 and their best 20: 206 us against 239; f32, whose rows take twice the
+// time to stream, gains nothing (247 us against 234 on 2048 x 151936 with 64), nor do fewer rows than blocks, and from some
+// 64 on the candidates are too many for 256 threads.
+template <typename T, int G>
 static int32_t launch_scores(mtb200_ctx* h, const ScoreArgs& a) {
-  void (*kernel)(ScoreArgs) = a.top ? (a.entropy ? token_scores_kernel<T, THREADS, true, true> : token_scores_kernel<T, THREADS, true, false>)
-                                    : (a.entropy ? token_scores_kernel<T, THREADS, false, true> : token_scores_kernel<T, THREADS, false, false>);
-  MTB_CUDA(launch_rows(h, kernel, a.rows, a.parts, THREADS, a));
-  return MTB200_OK;
+  size_t smem = 0;
+  if constexpr (G == 512)
+    if (a.top && a.top <= 64 && sizeof(T) == 2 && a.rows > 2 * h->sm_count) return launch_scores<T, 256>(h, a);
+  if (a.top) smem = sizeof(TopScratch<G>) * Block<G>::ROWS + (a.parts > 1 ? sizeof(unsigned long long) * a.parts * a.top : 0);
+  return launch_rows<G>(h, a.top ? (a.entropy ? token_scores_kernel<T, G, true, true> : token_scores_kernel<T, G, true, false>)
+                                 : (a.entropy ? token_scores_kernel<T, G, false, true> : token_scores_kernel<T, G, false, false>),
+                        a, true, smem);
 }
-// The gradient kernels' blocks do not meet: a plain grid.
-template <typename T>
+template <typename T, int G>
 static int32_t launch_score_grad(mtb200_ctx* h, const ScoreGradArgs& a) {
-  const unsigned blocks = unsigned(a.rows) * unsigned(a.parts);
-  if (a.d_entropy) token_scores_grad_kernel<T, 512, true><<<blocks, 512, 0, h->stream>>>(a);
-  else token_scores_grad_kernel<T, 512, false><<<blocks, 512, 0, h->stream>>>(a);
-  MTB_CUDA(cudaGetLastError());
-  return MTB200_OK;
+  return launch_rows<G>(h, a.d_entropy ? token_scores_grad_kernel<T, G, true> : token_scores_grad_kernel<T, G, false>, a, false);
 }
-template <typename T>
-static int32_t launch_distill(mtb200_ctx* h, const DistillArgs& a, bool forward) {
-  if (forward) {
-    MTB_CUDA(launch_rows(h, a.dlogits ? distill_kernel<T, 512, true> : distill_kernel<T, 512, false>, a.rows, a.parts, 512, a));
-  } else {
-    distill_grad_kernel<T, 512><<<unsigned(a.rows) * unsigned(a.parts), 512, 0, h->stream>>>(a);
-    MTB_CUDA(cudaGetLastError());
-  }
-  return MTB200_OK;
+template <typename T, int G>
+static int32_t launch_distill(mtb200_ctx* h, const DistillArgs& a) {
+  if (!a.row_loss) return launch_rows<G>(h, distill_grad_kernel<T, G>, a, false);
+  return launch_rows<G>(h, a.dlogits ? distill_kernel<T, G, true> : distill_kernel<T, G, false>, a, true);
+}
+// f(element type, group size as a compile-time number)
+template <int G>
+struct GroupTag {};
+template <int G>
+constexpr int group_of(GroupTag<G>) {
+  return G;
+}
+template <typename F>
+static int32_t by_type_and_group(int32_t dtype, int group, F f) {
+  auto with = [&](auto element) {
+    return group == 32 ? f(element, GroupTag<32>()) : group == 128 ? f(element, GroupTag<128>()) : f(element, GroupTag<512>());
+  };
+  if (dtype == MTB200_F32) return with(float());
+  if (dtype == MTB200_F16) return with(__half());
+  return with(__nv_bfloat16());
 }
 static int same_phase(const void* x, const void* y) {
   return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
@@ -475,10 +558,9 @@ int32_t mtb200_token_log_probs(mtb200_handle h, int32_t dtype, int64_t rows, int
   a.inv_t = float(1.0 / temperature); a.c = float(1.4426950408889634 / temperature);
   a.log_probs = tokens ? log_probs : nullptr; a.entropy = entropy; a.top_log_probs = top_log_probs;
   a.top_indices = top_indices; a.stats = stats; a.bad_label = h->status + 1;
-  a.parts = row_parts(h, rows, vocab * int64_t(logit_size(dtype)));
-  if (dtype == MTB200_F32) return launch_scores<float, 512>(h, a);
-  if (dtype == MTB200_F16) return launch_scores<__half, 512>(h, a);
-  return launch_scores<__nv_bfloat16, 512>(h, a);
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), TopScratch<32>::MOST, TopScratch<128>::MOST, top);
+  a.parts = plan.parts;
+  return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_scores<decltype(element), group_of(tag)>(h, a); });
 }
 
 int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
@@ -505,16 +587,15 @@ int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows,
   a.stats = stats; a.entropy = entropy; a.d_log_probs = d_log_probs; a.d_entropy = d_entropy; a.d_top = d_top;
   a.top_indices = top_indices; a.bad_label = h->status + 1;
   a.same_phase = same_phase(logits, dlogits);
-  a.parts = row_parts(h, rows, vocab * int64_t(logit_size(dtype)));
-  if (dtype == MTB200_F32) return launch_score_grad<float>(h, a);
-  if (dtype == MTB200_F16) return launch_score_grad<__half>(h, a);
-  return launch_score_grad<__nv_bfloat16>(h, a);
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), VOCAB_TOP_MAX, VOCAB_TOP_MAX, top);
+  a.parts = plan.parts;
+  return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_score_grad<decltype(element), group_of(tag)>(h, a); });
 }
 
 static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, int64_t rows, int64_t vocab, const void* logits,
                             int64_t ld, int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
                             int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
-                            const float* upstream_rows, void* dlogits, DistillArgs* a) {
+                            const float* upstream_rows, void* dlogits, DistillArgs* a, int* group) {
   if (int32_t rc = check_rows(what, dtype, rows, vocab, logits, ld, temperature)) return rc;
   if (int32_t rc = check_index(what, index_dtype)) return rc;
   if (!logit_size(teacher_dtype))
@@ -535,7 +616,9 @@ static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, in
   a->scale = float(temperature * (reduction == MTB200_REDUCE_MEAN && rows ? 1.0 / double(rows) : 1.0) * double(upstream));
   a->upstream_rows = upstream_rows; a->bad_label = h->status + 1;
   a->same_phase = same_phase(logits, dlogits);
-  a->parts = row_parts(h, rows, vocab * int64_t(logit_size(dtype)));
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), TEACHER_WARP_MAX, VOCAB_TEACHER_MAX, top);
+  a->parts = plan.parts;
+  *group = plan.group;
   return MTB200_OK;
 }
 
@@ -545,8 +628,9 @@ int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t voc
                        float* loss, float* stats, void* dlogits) {
   MTB_CHECK_HANDLE(h);
   DistillArgs a;
+  int group;
   if (int32_t rc = distill_args(h, "distill", dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype, teacher_logits,
-                                teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a))
+                                teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a, &group))
     return rc;
   if ((rows > 0 && !row_loss) || (reduction != MTB200_REDUCE_NONE && !loss)) return fail(MTB200_ERR_INVALID, "null loss pointer");
   a.row_loss = row_loss;
@@ -556,8 +640,8 @@ int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t voc
       if (top) return fail(MTB200_ERR_INVALID, "distill: empty vocabulary");
       MTB_CUDA(cudaMemsetAsync(row_loss, 0, sizeof(float) * size_t(rows), h->stream));
     } else {
-      int32_t rc = dtype == MTB200_F32 ? launch_distill<float>(h, a, true)
-                   : dtype == MTB200_F16 ? launch_distill<__half>(h, a, true) : launch_distill<__nv_bfloat16>(h, a, true);
+      const int32_t rc = by_type_and_group(
+          dtype, group, [&](auto element, auto tag) { return launch_distill<decltype(element), group_of(tag)>(h, a); });
       if (rc) return rc;
     }
   }
@@ -576,14 +660,15 @@ int32_t mtb200_distill_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t
                            const float* upstream_rows, const float* stats, void* dlogits) {
   MTB_CHECK_HANDLE(h);
   DistillArgs a;
+  int group;
   if (int32_t rc = distill_args(h, "distill_bwd", dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype,
-                                teacher_logits, teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a))
+                                teacher_logits, teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a, &group))
     return rc;
   if (rows == 0 || vocab == 0) return MTB200_OK;
   if (!stats || !dlogits) return fail(MTB200_ERR_INVALID, "distill_bwd: null pointer");
   a.stats = const_cast<float*>(stats);
-  return dtype == MTB200_F32 ? launch_distill<float>(h, a, false)
-         : dtype == MTB200_F16 ? launch_distill<__half>(h, a, false) : launch_distill<__nv_bfloat16>(h, a, false);
+  return by_type_and_group(dtype, group,
+                           [&](auto element, auto tag) { return launch_distill<decltype(element), group_of(tag)>(h, a); });
 }
 
 }  // extern "C"

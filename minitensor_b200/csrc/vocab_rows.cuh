@@ -29,6 +29,26 @@ __device__ __forceinline__ float ex2_ftz(float x) {
   return y;
 }
 
+// Two f32 operations per instruction, each rounded as its scalar form.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 // ------------------------------------------------------------------ element types
 template <typename T>
 struct LogitType;
@@ -41,6 +61,12 @@ struct LogitType<float> {
   static __device__ __forceinline__ float down(float x) { return x; }
   static __device__ __forceinline__ void unpack(const uint4& w, float (&f)[4]) {
     f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ float most(const uint4& w) {  // NaN counts as nothing
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ float least(const uint4& w) {
+    return fminf(fminf(__uint_as_float(w.x), __uint_as_float(w.y)), fminf(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
@@ -60,6 +86,16 @@ struct LogitType<__nv_bfloat16> {
       f[2 * i] = __uint_as_float(u[i] << 16);
       f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
+  }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float least(const uint4& w) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    return fminf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t u[4];
@@ -87,6 +123,16 @@ struct LogitType<__half> {
       f[2 * i + 1] = p.y;
     }
   }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float least(const uint4& w) {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+    const __half2 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    return fminf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t u[4];
 #pragma unroll
@@ -98,9 +144,23 @@ struct LogitType<__half> {
   }
 };
 
-// The part of one row that one block works on.  Only whole 16-byte vectors inside the row are read as vectors; the
+// The threads that work on one row (or on one part of it): a warp, or the whole block.
+template <int G>
+struct Group {
+  static constexpr int WARPS = G / 32;
+  static __device__ __forceinline__ int rank() { return G == 32 ? threadIdx.x & 31 : threadIdx.x; }
+  static __device__ __forceinline__ void sync() {
+    if (G == 32) __syncwarp();
+    else __syncthreads();
+  }
+  static __device__ __forceinline__ int count(bool b) {  // threads that say yes; a barrier
+    return G == 32 ? __popc(__ballot_sync(0xffffffffu, b)) : __syncthreads_count(b);
+  }
+};
+
+// The part of one row that one group works on.  Only whole 16-byte vectors inside the row are read as vectors; the
 // elements before the first boundary (`head`) belong to the row's first part and those after the last one (`tail`)
-// to its last part, and are read one by one.  Thread t owns head element t, the vectors v0 + t, v0 + t + THREADS,
+// to its last part, and are read one by one.  Thread t of G owns head element t, the vectors v0 + t, v0 + t + G,
 // ... and tail element t: its "unit", in ascending order of index.
 template <typename T>
 struct RowPart {
@@ -137,127 +197,8 @@ __device__ __forceinline__ bool owns(const RowPart<T>& p, int j) {
   return v >= p.v0 && v < p.v1;
 }
 
-// ------------------------------------------------------------------ statistics
-struct RowStat {
-  float m, s, u;
-};
-// Both orders of a merge give the same exponents, and -inf with -inf (or +inf with +inf) must not turn 0 into NaN:
-// the difference is clamped to the largest finite magnitude, whose power of two is 0; a NaN sum survives the product.
-__device__ __forceinline__ RowStat merge(const RowStat& a, const RowStat& b, float c) {
-  RowStat r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - r.m, -FLT_MAX), db = fmaxf(b.m - r.m, -FLT_MAX);
-  const float ra = ex2_ftz(da * c), rb = ex2_ftz(db * c);
-  r.s = a.s * ra + b.s * rb;
-  // a part that is scaled to nothing drops out (0 * -FLT_MAX is fine, an overflowed s * d is not)
-  r.u = (ra == 0.0f ? a.s * 0.0f : ra * (a.u + a.s * da)) + (rb == 0.0f ? b.s * 0.0f : rb * (b.u + b.s * db));
-  return r;
-}
-
-constexpr int ROW_UNROLL = 4;  // vectors a thread keeps in flight
-
-// The thread's unit, reduced.  `where` names the place of the unit's first maximum for find_first: the base vector
-// of its group of ROW_UNROLL vectors, or WHERE_HEAD / WHERE_TAIL / WHERE_START (nothing above -inf was seen).
-constexpr int WHERE_START = -1, WHERE_HEAD = -2, WHERE_TAIL = -3;
-
-template <bool ENT, int E>
-__device__ __forceinline__ void accumulate(const float (&x)[E], float c, RowStat& st, int& where, int here) {
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < E; ++i) top = fmaxf(top, x[i]);
-  if (top > st.m) {
-    const float d = fmaxf(st.m - top, -FLT_MAX);
-    const float r = ex2_ftz(d * c);
-    if (ENT) st.u = r == 0.0f ? st.s * 0.0f : r * (st.u + st.s * d);
-    st.s *= r;
-    st.m = top;
-    where = here;
-  }
-  const float base = st.m == -INFINITY ? 0.0f : st.m;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float d = x[i] - base;
-    const float e = ex2_ftz(d * c);
-    st.s += e;
-    if (ENT) st.u = fmaf(e, fmaxf(d, -FLT_MAX), st.u);
-  }
-}
-
-template <typename T, int THREADS, bool ENT>
-__device__ __forceinline__ RowStat unit_stats(const RowPart<T>& p, float c, int& where) {
-  using L = LogitType<T>;
-  constexpr int VEC = L::VEC;
-  const int tid = threadIdx.x;
-  RowStat st = {-INFINITY, 0.0f, 0.0f};
-  where = WHERE_START;
-  if (tid < p.head) {
-    const float x[1] = {L::up(p.row[tid])};
-    accumulate<ENT>(x, c, st, where, WHERE_HEAD);
-  }
-  const uint4* vecs = p.vecs();
-  for (int v = p.v0 + tid; v < p.v1; v += THREADS * ROW_UNROLL) {
-    uint4 w[ROW_UNROLL];
-#pragma unroll
-    for (int k = 0; k < ROW_UNROLL; ++k)
-      w[k] = v + k * THREADS < p.v1 ? vecs[v + k * THREADS]
-                                    : make_uint4(L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD);
-    float x[ROW_UNROLL * VEC];
-#pragma unroll
-    for (int k = 0; k < ROW_UNROLL; ++k) {
-      float f[VEC];
-      L::unpack(w[k], f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[k * VEC + i] = f[i];
-    }
-    accumulate<ENT>(x, c, st, where, v);
-  }
-  if (tid < p.tail) {
-    const float x[1] = {L::up(p.row[p.tail_base + tid])};
-    accumulate<ENT>(x, c, st, where, WHERE_TAIL);
-  }
-  return st;
-}
-
-// Block-wide merge in a fixed order; every thread returns the result.  `sm` holds THREADS / 32 + 1 entries.
-template <int THREADS>
-__device__ __forceinline__ RowStat block_merge(RowStat st, float c, RowStat* sm) {
-  constexpr int WARPS = THREADS / 32;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    RowStat other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.u = __shfl_xor_sync(0xffffffffu, st.u, o);
-    st = merge(st, other, c);
-  }
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = st;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    st = threadIdx.x < WARPS ? sm[threadIdx.x] : RowStat{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      RowStat other;
-      other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-      other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-      other.u = __shfl_xor_sync(0xffffffffu, st.u, o);
-      st = merge(st, other, c);
-    }
-    if (threadIdx.x == 0) sm[WARPS] = st;
-  }
-  __syncthreads();
-  return sm[WARPS];
-}
-
-// The row's statistics from those of the cluster's blocks, merged in rank order (the same bits in every block).
-// `mine` is in shared memory; the caller keeps it alive until its own last cluster barrier.
-__device__ __forceinline__ RowStat cluster_merge(cg::cluster_group& cluster, RowStat* mine, int parts, float c) {
-  RowStat st = *cluster.map_shared_rank(mine, 0);
-  for (int r = 1; r < parts; ++r) st = merge(st, *cluster.map_shared_rank(mine, r), c);
-  return st;
-}
-
-// ------------------------------------------------------------------ the largest entries
-// Order of the selection: larger logit first, ties to the lower index, -0 = +0, NaN ranks with -inf.  A candidate is
+// ------------------------------------------------------------------ order of the selection
+// Larger logit first, ties to the lower index, -0 = +0, NaN ranks with -inf.  A candidate is
 // one 64-bit word, the order-preserving image of the logit above the complement of the index; larger is better, no
 // two are equal, and 0 is no candidate.
 __device__ __forceinline__ uint32_t rank_key(float x) {
@@ -276,157 +217,404 @@ __device__ __forceinline__ int candidate_index(unsigned long long w) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(w));
 }
 
-constexpr int TOP_CAPACITY = 2304;  // candidates the buffer holds: 256 units of one 8-element vector, head and tail
-template <int THREADS>
-struct TopScratch {
-  unsigned long long pool[TOP_CAPACITY];
-  unsigned long long best[VOCAB_TOP_MAX];  // the part's result, best first
-  int hot[THREADS];
-  int hot_count, pool_count;
+// ------------------------------------------------------------------ statistics
+struct RowStat {
+  float m, s, u;
+};
+// The same sums relative to another, not smaller maximum.  -inf from -inf (or +inf from +inf) must not turn 0 into NaN: the
+// difference is clamped to the largest finite magnitude, whose power of two is 0.  Sums that are scaled to nothing drop out
+// whole (0 * (s * d) could be 0 * inf); a NaN stays.
+__device__ __forceinline__ void rescale(float from, float to, float c, float& s, float& u) {
+  const float d = fmaxf(from - to, -FLT_MAX);
+  const float r = ex2_ftz(d * c);
+  u = r == 0.0f ? s * 0.0f : r * fmaf(s, d, u);
+  s *= r;
+}
+// Merge over the lanes of a warp, in a fixed order; every lane returns it.
+__device__ __forceinline__ RowStat warp_merge(RowStat st, float c) {
+  const float m = key_value(__reduce_max_sync(0xffffffffu, rank_key(st.m)));
+  rescale(st.m, m, c, st.s, st.u);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+    st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
+  }
+  st.m = m;
+  return st;
+}
+
+// Vectors a thread takes up together, in one round: four loads in flight.
+constexpr int ROW_UNROLL = 4;
+
+// For the selection, a part's vectors are cut into at most SLOTS spans per thread, and the upper half of the largest
+// key of each span is kept.
+constexpr int SLOTS = 16;
+template <int G>
+struct Spans {
+  static constexpr int U = ROW_UNROLL;
+  static_assert(U == 4, "bits()");
+  int shift;  // a span is U << shift vectors of a unit
+  __device__ __forceinline__ explicit Spans(int vectors) {
+    const int rounds = (vectors + G * U - 1) / (G * U);
+    shift = rounds <= SLOTS ? 0 : 32 - __clz((rounds - 1) / SLOTS);
+  }
+  __device__ __forceinline__ int size() const { return U << shift; }
+  __device__ __forceinline__ int bits() const { return shift + 2; }
 };
 
-// Index of the unit's first element whose key is `key`, in the group `where` that unit_stats recorded.
-template <typename T, int THREADS>
-__device__ __forceinline__ int find_first(const RowPart<T>& p, int where, uint32_t key) {
-  using L = LogitType<T>;
-  constexpr int VEC = L::VEC;
-  const int tid = threadIdx.x;
-  if (where == WHERE_HEAD) return tid;
-  if (where == WHERE_TAIL) return p.tail_base + tid;
-  if (where == WHERE_START) {  // nothing above -inf: the unit's first element
-    if (tid < p.head) return tid;
-    if (p.v0 + tid < p.v1) return p.vec_base + (p.v0 + tid) * VEC;
-    return p.tail_base + tid;
+// A thread's running sums; the pairs are two independent halves.  `where` is the vector that holds the unit's first
+// maximum, or WHERE_HEAD / WHERE_TAIL / WHERE_START (nothing above -inf was seen).
+constexpr int WHERE_START = -1, WHERE_HEAD = -2, WHERE_TAIL = -3;
+struct UnitStat {
+  float m;
+  float2 s, u;
+  int where;
+  __device__ __forceinline__ RowStat sum() const { return {m, s.x + s.y, u.x + u.y}; }
+};
+__device__ __forceinline__ void raise_max(UnitStat& st, float top, float c) {
+  rescale(st.m, top, c, st.s.x, st.u.x);
+  rescale(st.m, top, c, st.s.y, st.u.y);
+  st.m = top;
+}
+template <bool ENT>
+__device__ __forceinline__ void add_one(UnitStat& st, float x, float c, int here) {
+  if (x > st.m) {
+    raise_max(st, x, c);
+    st.where = here;
   }
-  int found = INT_MAX;
-  for (int k = 0; k < ROW_UNROLL; ++k) {
-    const int v = where + k * THREADS;
-    if (v >= p.v1) break;
-    float f[VEC];
-    L::unpack(p.vecs()[v], f);
+  const float d = x - (st.m == -INFINITY ? 0.0f : st.m);
+  const float e = ex2_ftz(d * c);
+  st.s.x += e;
+  if (ENT) st.u.x = fmaf(e, fmaxf(d, -FLT_MAX), st.u.x);
+}
+// CLEAN: no difference is -inf (or the row is NaN anyway)
+template <typename T, bool ENT, bool CLEAN>
+__device__ __forceinline__ void add_vector(float2& s, float2& u, const uint4& w, float base, float c) {
+  using L = LogitType<T>;
+  float f[L::VEC];
+  L::unpack(w, f);
+  const float2 nb = make_float2(-base, -base), cc = make_float2(c, c);
 #pragma unroll
-    for (int i = VEC - 1; i >= 0; --i)
-      if (rank_key(f[i]) == key) found = min(found, p.vec_base + v * VEC + i);
-    if (found != INT_MAX) break;
-  }
-  return found;
-}
-
-// The best `count` of pool[0, n) into best[0, count) in order, by counting for each candidate those above it.
-template <int THREADS>
-__device__ __forceinline__ void rank_pool(const unsigned long long* pool, int n, int count, unsigned long long* best) {
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const unsigned long long w = pool[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += pool[j] > w;
-    if (above < count) best[above] = w;
-  }
-}
-
-// The `top` best candidates of the block's part into ts.best (0 where the part has fewer).  Every unit's maximum is
-// known from the statistics pass.  The top-th largest of those maxima bounds the top-th largest element from below,
-// and only the `top` units whose maximum reaches the bound can hold an element that does: those units alone are read
-// again (from L2), a warp per unit.  For values without order in the index some top + top^2 / (2 THREADS) elements
-// pass.  Where so many pass that the pool overflows, it is cut to the best `top` between steps and the bound raised.
-// Ends with a block barrier.
-template <typename T, int THREADS>
-__device__ void select_top(const RowPart<T>& p, int top, float unit_max, int where, TopScratch<THREADS>& ts) {
-  using L = LogitType<T>;
-  constexpr int VEC = L::VEC, SHIFT = L::KEY_SHIFT;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool any = tid < p.head || p.v0 + tid < p.v1 || tid < p.tail;
-  const uint32_t key = any ? rank_key(unit_max) >> SHIFT : 0u;
-  if (tid == 0) ts.hot_count = ts.pool_count = 0;
-  for (int i = tid; i < top; i += THREADS) ts.best[i] = 0ull;
-  // largest bound that `top` units reach (0: there are fewer units than that)
-  uint32_t bound = 0;
-  for (int b = 31 - SHIFT; b >= 0; --b) {
-    const uint32_t t = bound | (1u << b);
-    if (__syncthreads_count(key >= t) >= top) bound = t;
-  }
-  bool hot = any && key >= bound;
-  int last = INT_MAX;  // among elements equal to the bound, the largest index that may count
-  if (bound) {
-    const int above = __syncthreads_count(key > bound), equal = __syncthreads_count(key == bound);
-    if (above + equal > top) {  // ties: those units whose first such element comes first
-      const int first = key == bound ? find_first<T, THREADS>(p, where, rank_key(unit_max)) : INT_MAX;
-      const int want = top - above;
-      last = 0;  // smallest index that `want` of the tied units do not exceed
-      for (int b = 30; b >= 0; --b) {
-        const int t = last | ((1 << b) - 1);  // all indices with this prefix and bit b clear
-        if (__syncthreads_count(key == bound && first <= t) < want) last |= 1 << b;
-      }
-      hot = key > bound || (key == bound && first <= last);
+  for (int i = 0; i < L::VEC; i += 2) {
+    float2 d = add2(make_float2(f[i], f[i + 1]), nb);
+    const float2 g = mul2(d, cc);
+    const float2 e = make_float2(ex2_ftz(g.x), ex2_ftz(g.y));
+    s = add2(s, e);
+    if (ENT) {
+      if (!CLEAN) d = make_float2(fmaxf(d.x, -FLT_MAX), fmaxf(d.y, -FLT_MAX));
+      u = fma2(e, d, u);
     }
   }
-  // the key's low SHIFT bits follow its sign bit: all ones below zero, all zeros from zero on
-  const uint32_t full = SHIFT && bound < (1u << (31 - SHIFT)) ? (bound << SHIFT) | ((1u << SHIFT) - 1u) : bound << SHIFT;
-  unsigned long long floor_w = bound ? candidate(full, last) : 1ull;
-  if (hot) ts.hot[atomicAdd(&ts.hot_count, 1)] = tid;
-  __syncthreads();
+}
+
+template <typename T, int G, bool ENT, bool TOP>
+__device__ __forceinline__ UnitStat unit_stats(const RowPart<T>& p, float c, uint16_t (*slots)[G]) {
+  using L = LogitType<T>;
+  constexpr int U = ROW_UNROLL;
+  const int tid = Group<G>::rank();
+  const Spans<G> spans(p.v1 - p.v0);
+  float span_top = -INFINITY;
+  int round = 0;
+  UnitStat st = {-INFINITY, {0.0f, 0.0f}, {0.0f, 0.0f}, WHERE_START};
+  if (tid < p.head) add_one<ENT>(st, L::up(p.row[tid]), c, WHERE_HEAD);
+  const uint4* vecs = p.vecs();
+#pragma unroll 1  // a second round's loads would cost the registers of another block
+  for (int v = p.v0 + tid; v < p.v1; v += G * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      w[k] = v + k * G < p.v1 ? vecs[v + k * G]
+                              : make_uint4(L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD);
+    float most[U], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < U; ++k) top = fmaxf(top, most[k] = L::most(w[k]));
+    if (top > st.m) {
+      raise_max(st, top, c);
+      if (TOP) {
+#pragma unroll
+        for (int k = U - 1; k >= 0; --k)
+          if (most[k] == top) st.where = v + k * G;
+      }
+    }
+    if (TOP) {
+      span_top = fmaxf(span_top, top);
+      ++round;
+      if ((round & ((1 << spans.shift) - 1)) == 0 || v + G * U >= p.v1) {
+        slots[(round - 1) >> spans.shift][tid] = static_cast<uint16_t>(rank_key(span_top) >> 16);
+        span_top = -INFINITY;
+      }
+    }
+    const float base = st.m == -INFINITY ? 0.0f : st.m;
+    bool clean = true;
+    if (ENT) {
+      float low = INFINITY;
+#pragma unroll
+      for (int k = 0; k < U; ++k) low = fminf(low, L::least(w[k]));
+      clean = low - base > -INFINITY;  // else a masked element, or finite ones too far apart
+    }
+    if (clean) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) add_vector<T, ENT, true>(st.s, st.u, w[k], base, c);
+    } else {
+#pragma unroll
+      for (int k = 0; k < U; ++k) add_vector<T, ENT, false>(st.s, st.u, w[k], base, c);
+    }
+  }
+  if (tid < p.tail) add_one<ENT>(st, L::up(p.row[p.tail_base + tid]), c, WHERE_TAIL);
+  return st;
+}
+
+// Merge over the group in a fixed order; every thread returns the result.  `sm` holds Group<G>::WARPS + 1 entries and
+// is not used for a warp.
+template <int G>
+__device__ __forceinline__ RowStat group_merge(RowStat st, float c, RowStat* sm) {
+  constexpr int WARPS = Group<G>::WARPS;
+  st = warp_merge(st, c);
+  if (G == 32) return st;
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = st;
+  Group<G>::sync();
+  if (threadIdx.x < 32) {
+    st = warp_merge(threadIdx.x < WARPS ? sm[threadIdx.x] : RowStat{-INFINITY, 0.0f, 0.0f}, c);
+    if (threadIdx.x == 0) sm[WARPS] = st;
+  }
+  Group<G>::sync();
+  return sm[WARPS];
+}
+
+// The row's statistics from those of its parts, merged in their order.
+__device__ __forceinline__ RowStat parts_merge(const RowStat* parts, int n, float c) {
+  RowStat st = {parts[0].m, 0.0f, 0.0f};
+  for (int q = 1; q < n; ++q) st.m = fmaxf(st.m, parts[q].m);
+  for (int q = 0; q < n; ++q) {
+    float s = parts[q].s, u = parts[q].u;
+    rescale(parts[q].m, st.m, c, s, u);
+    st.s += s;
+    st.u += u;
+  }
+  return st;
+}
+
+// ------------------------------------------------------------------ the largest entries
+template <int G>
+struct TopScratch {
+  static constexpr int MOST = G < VOCAB_TOP_MAX ? G : VOCAB_TOP_MAX;  // largest `top`
+  // A part with fewer units than `top` has at most one vector a unit and 14 single elements: 255 * 8 + 14 candidates for
+  // a block, 31 * 8 + 14 for a warp.
+  static constexpr int CAPACITY = G == 32 ? 384 : G < VOCAB_TOP_MAX ? 1152 : 2304;
+  // units looked at: `top` and a few more
+  static __host__ __device__ constexpr int limit(int top) { return top + top / 16 + 16; }
+  static constexpr int UNITS = limit(MOST) < G ? limit(MOST) : G;
+  unsigned long long pool[CAPACITY];
+  unsigned long long best[MOST];  // the part's result, best first
+  static constexpr int HITS = G;
+  int hot[UNITS];                 // the units looked at
+  int hits[HITS];                 // spans read again: unit | slot << 16
+  uint16_t slots[SLOTS][G];       // upper halves of the spans' largest keys
+  uint32_t nth[Group<G>::WARPS], most[Group<G>::WARPS];
+  int hot_count, hit_count, pool_count;
+};
+
+// Calls f(i, above) for each entry i of list[0, n) with the number of entries above it, from one thread each.  As many
+// threads as there are to spare share an entry.  Every thread of the group takes part.
+template <int G, typename F>
+__device__ __forceinline__ void for_each_rank(const unsigned long long* list, int n, F f) {
+  const int tid = Group<G>::rank();
+  const int bits = n > 1 ? max(0, min(5, __clz(n - 1) - __clz(G) - 1)) : 5;  // 1 << bits threads per entry: n << bits <= G
+  const int sub = tid & ((1 << bits) - 1);
+  for (int base = (tid & ~31) >> bits; base < n; base += G >> bits) {  // whole warps leave
+    const int i = base + ((tid & 31) >> bits);
+    const unsigned long long w = i < n ? list[i] : ~0ull;
+    int above = 0;
+#pragma unroll 4
+    for (int j = sub; j < n; j += 1 << bits) above += list[j] > w;
+    for (int o = (1 << bits) >> 1; o; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (i < n && sub == 0) f(i, above);
+  }
+}
+// The best `count` of pool[0, n) into best[0, count) in order: by counting, or where the block's threads can take one
+// candidate each and counting would take longer (n^2 / 128 steps of a warp against 45 exchanges), by a bitonic sort,
+// within a warp by shuffles and across warps through the pool itself.  Every thread of the group takes part.
+template <int G>
+__device__ __forceinline__ void rank_pool(unsigned long long* pool, int n, int count, unsigned long long* best) {
+  if (G == 512 && n > 160 && n <= G) {
+    const int tid = threadIdx.x;
+    unsigned long long w = tid < n ? pool[tid] : 0ull;
+    for (int size = 2; size <= G; size <<= 1) {
+      const bool down = (tid & size) == 0 || size == G;
+      for (int o = size >> 1; o; o >>= 1) {
+        unsigned long long other;
+        if (o >= 32) {
+          Group<G>::sync();
+          pool[tid] = w;
+          Group<G>::sync();
+          other = pool[tid ^ o];
+        } else {
+          other = __shfl_xor_sync(0xffffffffu, w, o);
+        }
+        w = ((tid & o) == 0) == down ? max(w, other) : min(w, other);
+      }
+    }
+    if (tid < count) best[tid] = w;
+    return;
+  }
+  for_each_rank<G>(pool, n, [&](int i, int above) {
+    if (above < count) best[above] = pool[i];
+  });
+}
+
+// The `top` best candidates of the group's part into ts.best (0 where the part has fewer); top <= MOST.
+//  1. Every unit's maximum and its place are known from the statistics pass.  A key that at least `top` units reach bounds
+//     the top-th largest element from below: the least of the warps' ceil(top / warps)-th largest maxima.  Where many more
+//     units reach it, it is raised by bisection, and among units with equal keys by place, to just over `top` units.
+//  2. Only the units at or above the bound can hold an element that counts, and of those only the spans whose own largest
+//     key reaches it: these spans are read again.  For values without order in the index some r + r^2 / (2 G) elements of r
+//     units pass.  Where so many pass that the pool overflows, the units' vectors are gone through in rounds between
+//     which the pool is cut to the best `top` and the bound raised.
+//  3. Counting puts the candidates in order.
+// Ends with a group barrier.
+template <typename T, int G>
+__device__ void select_top(const RowPart<T>& p, int top, float unit_max, int where, TopScratch<G>& ts) {
+  using L = LogitType<T>;
+  constexpr int VEC = L::VEC, WARPS = Group<G>::WARPS, CAPACITY = TopScratch<G>::CAPACITY;
+  const int tid = Group<G>::rank(), lane = tid & 31, warp = tid >> 5;
+  const bool any = tid < p.head || p.v0 + tid < p.v1 || tid < p.tail;
+  const uint32_t key = any ? rank_key(unit_max) : 0u;
+  // the last index at which the unit's first maximum can be: a bound from below on its candidate word
+  int place;
+  if (where == WHERE_HEAD || (where == WHERE_START && tid < p.head)) place = tid;
+  else if (where == WHERE_TAIL || (where == WHERE_START && p.v0 + tid >= p.v1)) place = p.tail_base + tid;
+  else place = p.vec_base + (where == WHERE_START ? p.v0 + tid : where) * VEC + VEC - 1;
+  if (tid == 0) ts.hot_count = ts.hit_count = ts.pool_count = 0;
+  for (int i = tid; i < top; i += G) ts.best[i] = 0ull;
+
+  uint32_t low, high = __reduce_max_sync(0xffffffffu, key);
+  {
+    bool taken = false;
+    low = high;
+    for (int j = (top + WARPS - 1) / WARPS;;) {
+      const unsigned who = __ballot_sync(0xffffffffu, !taken && key == low);
+      if (--j == 0) break;
+      taken = taken || lane == __ffs(who) - 1;
+      low = __reduce_max_sync(0xffffffffu, taken ? 0u : key);
+    }
+  }
+  if (WARPS > 1) {
+    if (lane == 0) {
+      ts.nth[warp] = low;
+      ts.most[warp] = high;
+    }
+    Group<G>::sync();
+    low = __reduce_min_sync(0xffffffffu, lane < WARPS ? ts.nth[lane] : ~0u);
+    high = __reduce_max_sync(0xffffffffu, lane < WARPS ? ts.most[lane] : 0u);
+  }
+  low = max(low, 1u);  // 0 is no unit
+  const int limit = min(TopScratch<G>::limit(top), TopScratch<G>::UNITS);
+  int reach = Group<G>::count(key >= low);
+  int last = INT_MAX;  // of the units with key `low`, those up to this place
+  if (reach > limit) {
+    ++high;  // reached by none
+    while (reach > limit && high - low > 1) {
+      const uint32_t mid = low + (high - low) / 2;
+      const int c = Group<G>::count(key >= mid);
+      if (c >= top) {
+        low = mid;
+        reach = c;
+      } else {
+        high = mid;
+      }
+    }
+    if (reach > limit) {  // ties
+      const int want = top - Group<G>::count(key > low);
+      last = 0;  // becomes the smallest place that `want` of the tied units do not exceed
+      for (int b = 30; b >= 0; --b) {
+        const int t = last | ((1 << b) - 1);  // all places with this prefix and bit b clear
+        if (Group<G>::count(key == low && place <= t) < want) last |= 1 << b;
+      }
+    }
+  }
+  const bool hot = key > low || (key == low && place <= last);
+  unsigned long long floor_w = candidate(low, last);
+  {
+    const unsigned who = __ballot_sync(0xffffffffu, hot);
+    int at = 0;
+    if (lane == 0 && who) at = atomicAdd(&ts.hot_count, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+    if (hot) ts.hot[at] = tid;
+  }
+  Group<G>::sync();
   const int units = ts.hot_count;
 
-  auto visit = [&](int unit, int step) {  // lane's share of one step of 32 vectors of a unit
-    auto offer = [&](float x, int index) {
-      const unsigned long long w = candidate(rank_key(x), index);
-      if (w >= floor_w) {
-        const int at = atomicAdd(&ts.pool_count, 1);
-        if (at < TOP_CAPACITY) ts.pool[at] = w;
-      }
-    };
-    const int v = p.v0 + unit + (step * 32 + lane) * THREADS;
-    if (v < p.v1) {
-      float f[VEC];
-      L::unpack(p.vecs()[v], f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) offer(f[i], p.vec_base + v * VEC + i);
-    }
-    if (step == 0 && lane == 0) {
-      if (unit < p.head) offer(L::up(p.row[unit]), unit);
-      if (unit < p.tail) offer(L::up(p.row[p.tail_base + unit]), p.tail_base + unit);
+  auto offer = [&](float x, int index) {
+    const unsigned long long w = candidate(rank_key(x), index);
+    if (w >= floor_w) {
+      const int at = atomicAdd(&ts.pool_count, 1);
+      if (at < CAPACITY) ts.pool[at] = w;
     }
   };
-  const int steps = max(1, ((p.v1 - p.v0 + THREADS - 1) / THREADS + 31) / 32);
-  for (int i = warp; i < units * steps; i += THREADS / 32) visit(ts.hot[i / steps], i % steps);
-  __syncthreads();
+  const Spans<G> spans(p.v1 - p.v0);
+  auto passes = [&](int unit, int slot) { return ts.slots[slot][unit] >= static_cast<uint32_t>(floor_w >> 48); };
+  auto offer_vector = [&](const uint4& w, int v) {
+    float f[VEC];
+    L::unpack(w, f);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) offer(f[i], p.vec_base + v * VEC + i);
+  };
+  auto offer_singles = [&]() {
+    if (tid < p.head) offer(L::up(p.row[tid]), tid);
+    if (tid < p.tail) offer(L::up(p.row[p.tail_base + tid]), p.tail_base + tid);
+  };
+  const int each = (p.v1 - p.v0 + G - 1) / G;                           // vectors of a unit, some one less
+  const int span_bits = each > spans.size() ? 32 - __clz((each - 1) / spans.size()) : 0;  // spans per unit, a power of two
+  for (int i = tid; i < units << span_bits; i += G) {
+    const int unit = ts.hot[i >> span_bits], slot = i & ((1 << span_bits) - 1);
+    if (p.v0 + unit + slot * spans.size() * G < p.v1 && passes(unit, slot)) {
+      const int at = atomicAdd(&ts.hit_count, 1);
+      if (at < TopScratch<G>::HITS) ts.hits[at] = unit | slot << 16;
+    }
+  }
+  offer_singles();
+  Group<G>::sync();
+  const int hits = ts.hit_count;
+  if (hits <= TopScratch<G>::HITS) {
+    for (int i = tid; i < hits << spans.bits(); i += G) {
+      const int hit = ts.hits[i >> spans.bits()];
+      const int v = p.v0 + (hit & 0xffff) + ((hit >> 16) * spans.size() + (i & (spans.size() - 1))) * G;
+      if (v < p.v1) offer_vector(p.vecs()[v], v);
+    }
+  }
+  Group<G>::sync();
   int n = ts.pool_count;
-  if (n > TOP_CAPACITY) {
-    // a step offers at most 32 * VEC + 2 elements: as many warps at a time as the pool surely has room for
-    __syncthreads();
+  if (n > CAPACITY || hits > TopScratch<G>::HITS) {
+    // as many vectors at a time as the pool surely has room for beside the best
+    constexpr int ROOM = (CAPACITY - TopScratch<G>::MOST - 2 * VEC) / VEC;
+    constexpr int AT_ONCE = ROOM < G ? ROOM : G;
+    static_assert(AT_ONCE >= 1, "the pool must hold one vector beside the best");
+    Group<G>::sync();
     if (tid == 0) ts.pool_count = 0;
-    __syncthreads();
-    constexpr int AT_ONCE = (TOP_CAPACITY - VOCAB_TOP_MAX) / (32 * VEC + 2) < THREADS / 32
-                                ? (TOP_CAPACITY - VOCAB_TOP_MAX) / (32 * VEC + 2) : THREADS / 32;
-    for (int base = 0; base < units * steps; base += AT_ONCE) {
-      const int i = base + warp;
-      if (warp < AT_ONCE && i < units * steps) visit(ts.hot[i / steps], i % steps);
-      __syncthreads();
+    Group<G>::sync();
+    offer_singles();
+    const long long total = static_cast<long long>(units) * each;
+    for (long long base = 0; base < total; base += AT_ONCE) {
+      const long long i = base + tid;
+      if (tid < AT_ONCE && i < total) {
+        const int unit = ts.hot[i / each], j = static_cast<int>(i % each), v = p.v0 + unit + j * G;
+        if (v < p.v1 && passes(unit, j / spans.size())) offer_vector(p.vecs()[v], v);
+      }
+      Group<G>::sync();
       n = ts.pool_count;
-      __syncthreads();  // every thread has the same n before anyone offers more
-      if (n > TOP_CAPACITY - AT_ONCE * (32 * VEC + 2) && base + AT_ONCE < units * steps) {
-        rank_pool<THREADS>(ts.pool, n, top, ts.best);
-        __syncthreads();
-        for (int j = tid; j < top; j += THREADS) ts.pool[j] = ts.best[j];
+      Group<G>::sync();  // every thread has the same n before anyone offers more
+      if (n > CAPACITY - AT_ONCE * VEC && base + AT_ONCE < total) {
+        rank_pool<G>(ts.pool, n, top, ts.best);
+        Group<G>::sync();
+        for (int j = tid; j < top; j += G) ts.pool[j] = ts.best[j];
         if (tid == 0) ts.pool_count = top;
         floor_w = max(floor_w, ts.best[top - 1]);
-        __syncthreads();
+        Group<G>::sync();
       }
     }
-    n = ts.pool_count;
   }
-  rank_pool<THREADS>(ts.pool, n, top, ts.best);
-  __syncthreads();
-}
-
-// How many words of list[0, n), sorted best first, lie above `w`.
-__device__ __forceinline__ int count_above(const unsigned long long* list, int n, unsigned long long w) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] > w) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
+  rank_pool<G>(ts.pool, n, top, ts.best);
+  Group<G>::sync();
 }
 
 // ------------------------------------------------------------------ gradient pass
@@ -443,27 +631,28 @@ __device__ __forceinline__ float grad_at(float x, float c, const RowGrad& g) {
   // below 2^-1000 p is 0: the clamp keeps 0 * -inf out (a NaN comes through p)
   return ENT ? p * fmaf(g.b, fmaxf(lg, -1000.0f), g.a) : p * g.a;
 }
-template <typename T, int THREADS, bool ENT>
+constexpr int GRAD_UNROLL = 4;  // vectors a thread keeps in flight
+template <typename T, int G, bool ENT>
 __device__ __forceinline__ void dense_grad(const RowPart<T>& p, T* dx, float c, const RowGrad& g, bool same_phase) {
   using L = LogitType<T>;
-  constexpr int VEC = L::VEC;
-  const int tid = threadIdx.x;
+  constexpr int VEC = L::VEC, U = GRAD_UNROLL;
+  const int tid = Group<G>::rank();
   if (tid < p.head) dx[tid] = L::down(grad_at<ENT>(L::up(p.row[tid]), c, g));
   if (tid < p.tail) dx[p.tail_base + tid] = L::down(grad_at<ENT>(L::up(p.row[p.tail_base + tid]), c, g));
   const uint4* vecs = p.vecs();
-  for (int v = p.v0 + tid; v < p.v1; v += THREADS * ROW_UNROLL) {
-    uint4 w[ROW_UNROLL];
+  for (int v = p.v0 + tid; v < p.v1; v += G * U) {
+    uint4 w[U];
 #pragma unroll
-    for (int k = 0; k < ROW_UNROLL; ++k)
-      if (v + k * THREADS < p.v1) w[k] = vecs[v + k * THREADS];
+    for (int k = 0; k < U; ++k)
+      if (v + k * G < p.v1) w[k] = vecs[v + k * G];
 #pragma unroll
-    for (int k = 0; k < ROW_UNROLL; ++k) {
-      if (v + k * THREADS >= p.v1) continue;
+    for (int k = 0; k < U; ++k) {
+      if (v + k * G >= p.v1) continue;
       float f[VEC];
       L::unpack(w[k], f);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) f[i] = grad_at<ENT>(f[i], c, g);
-      T* out = dx + p.vec_base + (v + k * THREADS) * VEC;
+      T* out = dx + p.vec_base + (v + k * G) * VEC;
       if (same_phase) {
         *reinterpret_cast<uint4*>(out) = L::pack(f);
       } else {  // logits and gradient start at different offsets within 16 bytes
@@ -473,14 +662,14 @@ __device__ __forceinline__ void dense_grad(const RowPart<T>& p, T* dx, float c, 
     }
   }
 }
-template <typename T, int THREADS>
+template <typename T, int G>
 __device__ __forceinline__ void zero_grad(const RowPart<T>& p, T* dx, bool same_phase) {
   constexpr int VEC = LogitType<T>::VEC;
-  const int tid = threadIdx.x;
+  const int tid = Group<G>::rank();
   const T zero = LogitType<T>::down(0.0f);
   if (tid < p.head) dx[tid] = zero;
   if (tid < p.tail) dx[p.tail_base + tid] = zero;
-  for (int v = p.v0 + tid; v < p.v1; v += THREADS) {
+  for (int v = p.v0 + tid; v < p.v1; v += G) {
     T* out = dx + p.vec_base + v * VEC;
     if (same_phase) {
       *reinterpret_cast<uint4*>(out) = make_uint4(0u, 0u, 0u, 0u);
@@ -492,12 +681,12 @@ __device__ __forceinline__ void zero_grad(const RowPart<T>& p, T* dx, bool same_
 }
 // Entries (index, weight) added to the gradient: each is written once, as the rounding of dense value plus the sum of
 // all weights with its index, in list order (the same index may come several times).  idx < 0 marks no entry.  Runs
-// after the block barrier that follows dense_grad.
-template <typename T, int THREADS, bool ENT>
+// after the group barrier that follows dense_grad.
+template <typename T, int G, bool ENT>
 __device__ __forceinline__ void sparse_fix(const RowPart<T>& p, T* dx, float c, const RowGrad& g, const int* idx,
                                            const float* weight, int n) {
   using L = LogitType<T>;
-  for (int e = threadIdx.x; e < n; e += THREADS) {
+  for (int e = Group<G>::rank(); e < n; e += G) {
     const int j = idx[e];
     if (j < 0 || !owns(p, j)) continue;
     float w = 0.0f;
@@ -511,20 +700,22 @@ __device__ __forceinline__ void sparse_fix(const RowPart<T>& p, T* dx, float c, 
   }
 }
 
-// Row merging in small vectors: max and sum over the block, in a fixed order.  `sm`: THREADS / 32 floats.
-template <int THREADS, bool MAX>
-__device__ __forceinline__ float block_fold(float v, float* sm) {
+// Maximum or sum over the group, in a fixed order; every thread returns it.  `sm`: Group<G>::WARPS floats, not used for
+// a warp.
+template <int G, bool MAX>
+__device__ __forceinline__ float group_fold(float v, float* sm) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const float w = __shfl_xor_sync(0xffffffffu, v, o);
     v = MAX ? fmaxf(v, w) : v + w;
   }
-  __syncthreads();  // the previous use of sm is over
+  if (G == 32) return v;
+  Group<G>::sync();  // the previous use of sm is over
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
+  Group<G>::sync();
   v = sm[0];
 #pragma unroll
-  for (int k = 1; k < THREADS / 32; ++k) v = MAX ? fmaxf(v, sm[k]) : v + sm[k];
+  for (int k = 1; k < Group<G>::WARPS; ++k) v = MAX ? fmaxf(v, sm[k]) : v + sm[k];
   return v;
 }
 

@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # (rows, vocabulary, extra columns in memory): one token and one class, odd sizes, parts of a vector, several blocks a row
 SHAPES = [(1, 1, 0), (1, 2, 1), (3, 7, 0), (5, 8, 8), (9, 127, 3), (4, 1000, 0), (33, 4099, 13), (2, 32003, 61), (301, 6007, 1),
-          (700, 515, 0), (1, 200001, 7)]
+          (700, 515, 0), (1, 200001, 7), (320, 20001, 2)]
 
 
 def logits_for(rows, vocab, pad, dtype, seed, spread=2.5):
