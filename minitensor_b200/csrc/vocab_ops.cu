@@ -51,10 +51,10 @@ struct Block {
   static __device__ __forceinline__ int slot() { return G == 32 ? threadIdx.x >> 5 : 0; }
   // row index, or -1 behind the last one (then the whole group has nothing to do)
   static __device__ __forceinline__ long long row(int rows, int parts) {
-    const long long r = G == 32 ? static_cast<long long>(blockIdx.x) * ROWS + slot() : blockIdx.x / parts;
+    const long long r = G == 32 ? static_cast<long long>(blockIdx.x) * ROWS + slot() : blockIdx.x / static_cast<unsigned>(parts);
     return r < rows ? r : -1;
   }
-  static __device__ __forceinline__ int part(int parts) { return G == 32 ? 0 : blockIdx.x % parts; }
+  static __device__ __forceinline__ int part(int parts) { return G == 32 ? 0 : blockIdx.x % static_cast<unsigned>(parts); }
 };
 
 constexpr float LN2 = 0.693147180559945309f;
@@ -250,7 +250,7 @@ struct DistillArgs {
   float scale;             // T * reduction factor * upstream: d loss / d logits = scale * weight_r * (Q p - q)
   const float* upstream_rows;
   float *row_loss, *stats;
-  uint32_t* bad_label;
+  uint32_t *status, *bad_label;
 };
 
 constexpr int TEACHER_WARP_MAX = 128;  // entries where a warp has a row of its own: 12 KB a block
@@ -366,6 +366,142 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
     for (int e = tid; e < a.top; e += G) q[e] *= -scale;
     Group<G>::sync();
     sparse_fix<T, G, false>(p, dx, a.c, g, idx, q, a.top);
+  }
+}
+
+// Loss and gradient of long rows: a cluster per row, so that the rows in flight stay in L2 between the two looks at them
+// (2048 x 128256 f32 with a block per row: 493 us, as long as two reads and a write from HBM take).  A block's chain of steps
+// is short: its logits are asked for first; what a row needs once is done by one warp, what its entries need by the warps
+// that have entries (from the second on: thread 32 + e has entry e); and the parts exchange their statistics by messages
+// instead of a cluster barrier, which would wait for all memory operations under way.
+constexpr int CLUSTER_TEACHER = 480;  // entries
+template <typename T>
+static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillArgs a) {
+  using L = LogitType<T>;
+  constexpr int G = 512, WARPS = Group<G>::WARPS;
+  __shared__ RowStat stat_sm[WARPS], teacher_sm[WARPS];
+  __shared__ float4 parts_st[MAX_PARTS], row_sm;  // row_sm: m, ln S, whether there is no distribution
+  __shared__ __align__(8) unsigned long long arrived;
+  __shared__ float kl_sm[WARPS], weight[CLUSTER_TEACHER];
+  __shared__ int idx[CLUSTER_TEACHER], twice[CLUSTER_TEACHER];
+  __shared__ uint32_t never;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = tid - 32;
+  const bool entry = e >= 0 && e < a.top, entry_warp = warp > 0 && 32 * (warp - 1) < a.top;
+  const int part = Block<G>::part(a.parts);
+  const long long r = Block<G>::row(a.rows, a.parts);
+  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
+  T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
+  const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
+  if (tid == 0) {
+    mbar_init(smem_u32(&arrived), 1);
+    fence_mbar_init();
+    never = 0;
+  }
+  // The thread's entry.  The list is read before the logits are asked for: a row without an entry does not look at them.
+  int mine = -1;
+  float v = -INFINITY;
+  if (entry) {
+    const long long j = a.index.at(r * a.top + e);
+    if (j >= 0 && j < a.vocab) mine = static_cast<int>(j);
+    else if (j != -1 && part == 0) atomicOr(a.bad_label, 1u);
+    if (mine >= 0) v = a.value.at(r * a.top + e);
+    idx[e] = mine;
+    twice[e] = 0;
+  }
+  const bool live = Group<G>::count(v != -INFINITY) > 0;  // NaN counts: it has to reach the result
+  if (!live) {  // the same answer in every block of the cluster
+    if (part == 0 && tid == 0) {
+      a.row_loss[r] = 0.0f;
+      if (a.stats) {
+        a.stats[2 * r] = -INFINITY;
+        a.stats[2 * r + 1] = 0.0f;
+      }
+    }
+    zero_grad<T, G>(p, dx, a.same_phase);
+    return;
+  }
+  if (a.parts > 1) cluster.barrier_arrive();  // waited for before another block is sent to
+  const float scale = a.upstream_rows ? a.scale * a.upstream_rows[r] : a.scale;
+  const bool owner = mine >= 0 && owns(p, mine);
+  T x_mine = L::down(0.0f);
+  if (mine >= 0 && (owner || part == 0)) x_mine = row[mine];
+
+  const RowStat sum = warp_merge(unit_stats<T, G, false, false>(p, a.c, nullptr).sum(), a.c);
+  if (lane == 0) stat_sm[warp] = sum;
+  if (entry_warp) {
+    const RowStat st = warp_merge(RowStat{isnan(v) ? -INFINITY : v, v == -INFINITY ? 0.0f : 1.0f + (v - v), 0.0f}, a.c);
+    if (lane == 0) teacher_sm[warp] = st;
+  }
+  if (a.parts > 1) cluster.barrier_wait();
+  __syncthreads();
+  float q = 0.0f, dv = 0.0f, ln_sq = 0.0f;
+  if (warp == 0) {
+    RowStat st = warp_merge(lane < WARPS ? stat_sm[lane] : RowStat{-INFINITY, 0.0f, 0.0f}, a.c);
+    if (a.parts > 1) {
+      if (lane == 0) mbar_expect_tx(smem_u32(&arrived), uint32_t(a.parts) * 16u);
+      if (lane < a.parts) send_async(&parts_st[part], &arrived, lane, make_float4(st.m, st.s, 0.0f, 0.0f));
+      if (!mbar_wait(smem_u32(&arrived), 0, &never)) atomicMax(a.status, 0x1001u);
+      const float4 o = parts_st[lane < a.parts ? lane : 0];
+      st = warp_merge(lane < a.parts ? RowStat{o.x, o.y, 0.0f} : RowStat{-INFINITY, 0.0f, 0.0f}, a.c);
+    }
+    const bool none = st.m == -INFINITY && !isnan(st.s);
+    if (lane == 0) row_sm = make_float4(st.m, none ? 0.0f : logf(st.s), none ? 1.0f : 0.0f, 0.0f);
+  } else if (entry_warp) {
+    const bool used = lane > 0 && lane < WARPS && 32 * (lane - 1) < a.top;
+    const RowStat st = warp_merge(used ? teacher_sm[lane] : RowStat{-INFINITY, 0.0f, 0.0f}, a.c);
+    dv = v - (st.m == -INFINITY ? 0.0f : st.m);
+    q = ex2_ftz(dv * a.c) / st.s;
+    ln_sq = logf(st.s);
+    if (entry) weight[e] = -scale * q;
+  }
+  {
+    // Entries whose index stands in the list more than once (1: behind, 2: before), all threads sharing the work:
+    // 1 << shift threads have an entry each, and the next as many the rest of the list.
+    int shift = 0;
+    while ((1 << shift) < a.top) ++shift;
+    const int at = tid & ((1 << shift) - 1), others = G >> shift;
+    const int index = at < a.top ? idx[at] : -1;
+    if (index >= 0)
+      for (int k = tid >> shift; k < a.top; k += others)
+        if (idx[k] == index && k != at) atomicOr(&twice[at], k < at ? 2 : 1);
+  }
+  __syncthreads();
+  const float4 info = row_sm;
+  RowGrad g;
+  g.base = info.x == -INFINITY ? 0.0f : info.x;
+  g.l2 = info.y * LOG2E;
+  g.b = 0.0f;
+  bool teacher_nan = false;  // a NaN or +inf among the teacher's values is in the sum of its warp
+  for (int k = 1; k < WARPS && 32 * (k - 1) < a.top; ++k) teacher_nan = teacher_nan || isnan(teacher_sm[k].s);
+  g.a = teacher_nan ? NAN : scale;
+  dense_grad<T, G, false>(p, dx, a.c, g, a.same_phase);
+  if (entry_warp && part == 0) {
+    // log q - log p with the two maxima taken out first: nearly equal distributions lose nothing to the logarithms' size
+    float kl = 0.0f;
+    if (mine >= 0 && q != 0.0f) kl = q * ((dv - (info.z != 0.0f ? -INFINITY : L::up(x_mine) - info.x)) * a.inv_t - (ln_sq - info.y));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
+    if (lane == 0) kl_sm[warp] = kl;
+  }
+  __syncthreads();  // the dense gradient stands, with kl_sm
+  if (owner && !(twice[e] & 2)) {  // as sparse_fix, with the logit at hand
+    float w = weight[e];
+    if (twice[e]) {
+      w = 0.0f;
+      for (int k = 0; k < a.top; ++k)
+        if (idx[k] == mine) w += weight[k];
+    }
+    dx[mine] = L::down(grad_at<false>(L::up(x_mine), a.c, g) + w);
+  }
+  if (part == 0 && tid == 0) {
+    float kl = 0.0f;
+    for (int k = 1; k < WARPS && 32 * (k - 1) < a.top; ++k) kl += kl_sm[k];
+    a.row_loss[r] = a.t * a.t * kl;
+    if (a.stats) {
+      a.stats[2 * r] = info.x;
+      a.stats[2 * r + 1] = info.y;
+    }
   }
 }
 
@@ -500,8 +636,21 @@ template <typename T, int G>
 static int32_t launch_score_grad(mtb200_ctx* h, const ScoreGradArgs& a) {
   return launch_rows<G>(h, a.d_entropy ? token_scores_grad_kernel<T, G, true> : token_scores_grad_kernel<T, G, false>, a, false);
 }
+#ifndef DMB
+#define DMB 32
+#endif
+#ifndef DPB
+#define DPB 32768
+#endif
 template <typename T, int G>
 static int32_t launch_distill(mtb200_ctx* h, const DistillArgs& a) {
+  if constexpr (G == 512)
+    if (a.row_loss && a.dlogits && a.top <= CLUSTER_TEACHER) {
+      DistillArgs c = a;
+      const int64_t row_bytes = int64_t(a.vocab) * sizeof(T);
+      while (c.parts < MAX_PARTS && 3 * h->sm_count / c.parts * row_bytes > (DMB << 20) && row_bytes / (c.parts * 2) >= DPB) c.parts *= 2;
+      return launch_rows<G>(h, distill_cluster_kernel<T>, c, true);
+    }
   if (!a.row_loss) return launch_rows<G>(h, distill_grad_kernel<T, G>, a, false);
   return launch_rows<G>(h, a.dlogits ? distill_kernel<T, G, true> : distill_kernel<T, G, false>, a, true);
 }
@@ -614,7 +763,7 @@ static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, in
   a->value = {teacher_logits, teacher_dtype};
   a->t = float(temperature); a->inv_t = float(1.0 / temperature); a->c = float(1.4426950408889634 / temperature);
   a->scale = float(temperature * (reduction == MTB200_REDUCE_MEAN && rows ? 1.0 / double(rows) : 1.0) * double(upstream));
-  a->upstream_rows = upstream_rows; a->bad_label = h->status + 1;
+  a->upstream_rows = upstream_rows; a->status = h->status; a->bad_label = h->status + 1;
   a->same_phase = same_phase(logits, dlogits);
   const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), TEACHER_WARP_MAX, VOCAB_TEACHER_MAX, top);
   a->parts = plan.parts;

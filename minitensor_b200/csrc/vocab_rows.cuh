@@ -9,6 +9,7 @@
 // distribution: every logit -inf -> p = 0, log p = -inf, entropy 0;  a NaN or +inf -> NaN throughout.
 #pragma once
 #include "mtb200_core.cuh"
+#include "ptx_sm100.cuh"
 
 #include <cfloat>
 #include <climits>
@@ -27,6 +28,29 @@ __device__ __forceinline__ float ex2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 16 bytes from global to shared memory, both aligned, on the thread's own account: a group is what was asked for up to a
+// commit, and wait<N> returns when all groups but the last N have arrived, for the thread that asked.
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Four words into the shared memory of block `rank` of the cluster, at the place that `to` has in this block; they count on
+// the barrier of that block at the place of `bar`.
+__device__ __forceinline__ void send_async(const void* to, const unsigned long long* bar, int rank, float4 v) {
+  asm volatile(
+      "{\n\t.reg .b32 ra, rb;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tmapa.shared::cluster.u32 rb, %1, %2;\n\t"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [ra], {%3, %4, %5, %6}, [rb];\n\t}"
+      ::"r"(smem_u32(to)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)),
+      "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w))
+      : "memory");
 }
 
 // Two f32 operations per instruction, each rounded as its scalar form.
@@ -62,11 +86,22 @@ struct LogitType<float> {
   static __device__ __forceinline__ void unpack(const uint4& w, float (&f)[4]) {
     f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
   }
-  static __device__ __forceinline__ float most(const uint4& w) {  // NaN counts as nothing
-    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  // largest and least of N vectors; NaN counts as nothing
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4 (&w)[N]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(w[k].x), __uint_as_float(w[k].y)), fmaxf(__uint_as_float(w[k].z), __uint_as_float(w[k].w))));
+    return m;
   }
-  static __device__ __forceinline__ float least(const uint4& w) {
-    return fminf(fminf(__uint_as_float(w.x), __uint_as_float(w.y)), fminf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  template <int N>
+  static __device__ __forceinline__ float least(const uint4 (&w)[N]) {
+    float m = INFINITY;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      m = fminf(m, fminf(fminf(__uint_as_float(w[k].x), __uint_as_float(w[k].y)), fminf(__uint_as_float(w[k].z), __uint_as_float(w[k].w))));
+    return m;
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
@@ -87,14 +122,20 @@ struct LogitType<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ float most(const uint4& w) {
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4 (&w)[N]) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = __hmax2(m, __hmax2(__hmax2(h[4 * k], h[4 * k + 1]), __hmax2(h[4 * k + 2], h[4 * k + 3])));
     return fmaxf(__low2float(m), __high2float(m));
   }
-  static __device__ __forceinline__ float least(const uint4& w) {
+  template <int N>
+  static __device__ __forceinline__ float least(const uint4 (&w)[N]) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-    const __nv_bfloat162 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    __nv_bfloat162 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = __hmin2(m, __hmin2(__hmin2(h[4 * k], h[4 * k + 1]), __hmin2(h[4 * k + 2], h[4 * k + 3])));
     return fminf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
@@ -123,14 +164,20 @@ struct LogitType<__half> {
       f[2 * i + 1] = p.y;
     }
   }
-  static __device__ __forceinline__ float most(const uint4& w) {
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4 (&w)[N]) {
     const __half2* h = reinterpret_cast<const __half2*>(&w);
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = __hmax2(m, __hmax2(__hmax2(h[4 * k], h[4 * k + 1]), __hmax2(h[4 * k + 2], h[4 * k + 3])));
     return fmaxf(__low2float(m), __high2float(m));
   }
-  static __device__ __forceinline__ float least(const uint4& w) {
+  template <int N>
+  static __device__ __forceinline__ float least(const uint4 (&w)[N]) {
     const __half2* h = reinterpret_cast<const __half2*>(&w);
-    const __half2 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    __half2 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = __hmin2(m, __hmin2(__hmin2(h[4 * k], h[4 * k + 1]), __hmin2(h[4 * k + 2], h[4 * k + 3])));
     return fminf(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
@@ -180,8 +227,9 @@ __device__ __forceinline__ RowPart<T> row_part(const T* row, int n, int part, in
   const int nv = (n - head) / VEC;
   p.row = row;
   p.vec_base = head;
-  p.v0 = static_cast<int>(static_cast<long long>(nv) * part / parts);
-  p.v1 = static_cast<int>(static_cast<long long>(nv) * (part + 1) / parts);
+  const int share = static_cast<int>(static_cast<unsigned>(nv) / static_cast<unsigned>(parts)), more = nv - share * parts;
+  p.v0 = share * part + min(part, more);  // the first `more` parts have one vector more
+  p.v1 = p.v0 + share + (part < more);
   p.tail_base = head + nv * VEC;
   p.head = part == 0 ? head : 0;
   p.tail = part == parts - 1 ? n - p.tail_base : 0;
@@ -262,31 +310,38 @@ struct Spans {
   __device__ __forceinline__ int bits() const { return shift + 2; }
 };
 
-// A thread's running sums; the pairs are two independent halves.  `where` is the vector that holds the unit's first
-// maximum, or WHERE_HEAD / WHERE_TAIL / WHERE_START (nothing above -inf was seen).
+// A thread's running sums, relative to the maximum that its warp has met so far: that rises in few rounds (in the n-th
+// with probability 1 / n), where some lane's own maximum rises in nearly all of them.  The pairs are two independent
+// halves.  For the selection, m is the thread's own maximum and `where` the vector that holds it first, or WHERE_HEAD /
+// WHERE_TAIL / WHERE_START (nothing above -inf was seen).
 constexpr int WHERE_START = -1, WHERE_HEAD = -2, WHERE_TAIL = -3;
 struct UnitStat {
-  float m;
-  float2 s, u;
-  int where;
-  __device__ __forceinline__ RowStat sum() const { return {m, s.x + s.y, u.x + u.y}; }
-};
-__device__ __forceinline__ void raise_max(UnitStat& st, float top, float c) {
-  rescale(st.m, top, c, st.s.x, st.u.x);
-  rescale(st.m, top, c, st.s.y, st.u.y);
-  st.m = top;
-}
-template <bool ENT>
-__device__ __forceinline__ void add_one(UnitStat& st, float x, float c, int here) {
-  if (x > st.m) {
-    raise_max(st, x, c);
-    st.where = here;
+  float base = -INFINITY, m = -INFINITY;
+  float2 s = {0.0f, 0.0f}, u = {0.0f, 0.0f};
+  int where = WHERE_START;
+  __device__ __forceinline__ RowStat sum() const { return {base, s.x + s.y, u.x + u.y}; }
+  // by all lanes of the warp
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (!__any_sync(0xffffffffu, top > base)) return;
+    const float to = key_value(__reduce_max_sync(0xffffffffu, rank_key(fmaxf(top, base))));
+    rescale(base, to, c, s.x, u.x);
+    rescale(base, to, c, s.y, u.y);
+    base = to;
   }
-  const float d = x - (st.m == -INFINITY ? 0.0f : st.m);
-  const float e = ex2_ftz(d * c);
-  st.s.x += e;
-  if (ENT) st.u.x = fmaf(e, fmaxf(d, -FLT_MAX), st.u.x);
-}
+  __device__ __forceinline__ void own(float x, int here) {
+    if (x > m) {
+      m = x;
+      where = here;
+    }
+  }
+  template <bool ENT>
+  __device__ __forceinline__ void add_one(float x, float c) {  // x is not above base
+    const float d = x - (base == -INFINITY ? 0.0f : base);
+    const float e = ex2_ftz(d * c);
+    s.x += e;
+    if (ENT) u.x = fmaf(e, fmaxf(d, -FLT_MAX), u.x);
+  }
+};
 // CLEAN: no difference is -inf (or the row is NaN anyway)
 template <typename T, bool ENT, bool CLEAN>
 __device__ __forceinline__ void add_vector(float2& s, float2& u, const uint4& w, float base, float c) {
@@ -315,52 +370,67 @@ __device__ __forceinline__ UnitStat unit_stats(const RowPart<T>& p, float c, uin
   const Spans<G> spans(p.v1 - p.v0);
   float span_top = -INFINITY;
   int round = 0;
-  UnitStat st = {-INFINITY, {0.0f, 0.0f}, {0.0f, 0.0f}, WHERE_START};
-  if (tid < p.head) add_one<ENT>(st, L::up(p.row[tid]), c, WHERE_HEAD);
-  const uint4* vecs = p.vecs();
-#pragma unroll 1  // a second round's loads would cost the registers of another block
-  for (int v = p.v0 + tid; v < p.v1; v += G * U) {
-    uint4 w[U];
+  UnitStat st;
+  auto take = [&](const uint4 (&w)[U], int v) {  // one round of the whole warp
+    float top = -INFINITY;
+    if (TOP) {
+      float most[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      w[k] = v + k * G < p.v1 ? vecs[v + k * G]
-                              : make_uint4(L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD);
-    float most[U], top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < U; ++k) top = fmaxf(top, most[k] = L::most(w[k]));
-    if (top > st.m) {
-      raise_max(st, top, c);
-      if (TOP) {
+      for (int k = 0; k < U; ++k) {
+        const uint4 one[1] = {w[k]};
+        top = fmaxf(top, most[k] = L::most(one));
+      }
+      if (top > st.m) {
+        st.m = top;
 #pragma unroll
         for (int k = U - 1; k >= 0; --k)
           if (most[k] == top) st.where = v + k * G;
       }
-    }
-    if (TOP) {
       span_top = fmaxf(span_top, top);
       ++round;
       if ((round & ((1 << spans.shift) - 1)) == 0 || v + G * U >= p.v1) {
-        slots[(round - 1) >> spans.shift][tid] = static_cast<uint16_t>(rank_key(span_top) >> 16);
+        if (v < p.v1) slots[(round - 1) >> spans.shift][tid] = static_cast<uint16_t>(rank_key(span_top) >> 16);
         span_top = -INFINITY;
       }
+    } else {
+      top = L::most(w);
     }
-    const float base = st.m == -INFINITY ? 0.0f : st.m;
-    bool clean = true;
-    if (ENT) {
-      float low = INFINITY;
-#pragma unroll
-      for (int k = 0; k < U; ++k) low = fminf(low, L::least(w[k]));
-      clean = low - base > -INFINITY;  // else a masked element, or finite ones too far apart
-    }
-    if (clean) {
+    st.raise(top, c);
+    const float base = st.base == -INFINITY ? 0.0f : st.base;
+    // a masked element, or finite ones too far apart, make a difference of -inf
+    if (!ENT || L::least(w) - base > -INFINITY) {
 #pragma unroll
       for (int k = 0; k < U; ++k) add_vector<T, ENT, true>(st.s, st.u, w[k], base, c);
     } else {
 #pragma unroll
       for (int k = 0; k < U; ++k) add_vector<T, ENT, false>(st.s, st.u, w[k], base, c);
     }
+  };
+  if (TOP && tid < p.head) st.own(L::up(p.row[tid]), WHERE_HEAD);
+  const uint4* vecs = p.vecs();
+  int v = p.v0;
+#pragma unroll 1  // a second round's loads would cost the registers of another block
+  for (; v + G * U <= p.v1; v += G * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) w[k] = vecs[v + tid + k * G];
+    take(w, v + tid);
   }
-  if (tid < p.tail) add_one<ENT>(st, L::up(p.row[p.tail_base + tid]), c, WHERE_TAIL);
+  if (v < p.v1) {
+    uint4 w[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      w[k] = v + tid + k * G < p.v1 ? vecs[v + tid + k * G]
+                                    : make_uint4(L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD, L::NEG_INF_WORD);
+    take(w, v + tid);
+  }
+  if (TOP && tid < p.tail) st.own(L::up(p.row[p.tail_base + tid]), WHERE_TAIL);
+  if (p.head || p.tail) {
+    const float x = tid < p.head ? L::up(p.row[tid]) : -INFINITY, y = tid < p.tail ? L::up(p.row[p.tail_base + tid]) : -INFINITY;
+    st.raise(fmaxf(x, y), c);
+    if (tid < p.head) st.add_one<ENT>(x, c);
+    if (tid < p.tail) st.add_one<ENT>(y, c);
+  }
   return st;
 }
 
@@ -632,6 +702,28 @@ __device__ __forceinline__ float grad_at(float x, float c, const RowGrad& g) {
   return ENT ? p * fmaf(g.b, fmaxf(lg, -1000.0f), g.a) : p * g.a;
 }
 constexpr int GRAD_UNROLL = 4;  // vectors a thread keeps in flight
+template <typename T, bool ENT>
+__device__ __forceinline__ void grad_vector(T* out, const uint4& w, float c, const RowGrad& g, bool same_phase) {
+  using L = LogitType<T>;
+  float f[L::VEC];
+  L::unpack(w, f);
+  const float2 nb = make_float2(-g.base, -g.base), cc = make_float2(c, c), nl = make_float2(-g.l2, -g.l2);
+  const float2 ga = make_float2(g.a, g.a), gb = make_float2(g.b, g.b);
+#pragma unroll
+  for (int i = 0; i < L::VEC; i += 2) {  // grad_at, two at a time
+    const float2 lg = fma2(add2(make_float2(f[i], f[i + 1]), nb), cc, nl);
+    const float2 p = make_float2(ex2_ftz(lg.x), ex2_ftz(lg.y));
+    const float2 o = mul2(p, ENT ? fma2(gb, make_float2(fmaxf(lg.x, -1000.0f), fmaxf(lg.y, -1000.0f)), ga) : ga);
+    f[i] = o.x;
+    f[i + 1] = o.y;
+  }
+  if (same_phase) {
+    *reinterpret_cast<uint4*>(out) = L::pack(f);
+  } else {  // logits and gradient start at different offsets within 16 bytes
+#pragma unroll
+    for (int i = 0; i < L::VEC; ++i) out[i] = L::down(f[i]);
+  }
+}
 template <typename T, int G, bool ENT>
 __device__ __forceinline__ void dense_grad(const RowPart<T>& p, T* dx, float c, const RowGrad& g, bool same_phase) {
   using L = LogitType<T>;
@@ -639,27 +731,26 @@ __device__ __forceinline__ void dense_grad(const RowPart<T>& p, T* dx, float c, 
   const int tid = Group<G>::rank();
   if (tid < p.head) dx[tid] = L::down(grad_at<ENT>(L::up(p.row[tid]), c, g));
   if (tid < p.tail) dx[p.tail_base + tid] = L::down(grad_at<ENT>(L::up(p.row[p.tail_base + tid]), c, g));
-  const uint4* vecs = p.vecs();
-  for (int v = p.v0 + tid; v < p.v1; v += G * U) {
+  const uint4* vecs = p.vecs() + tid;
+  T* out = dx + p.vec_base + tid * VEC;
+  int v = p.v0;
+#pragma unroll 1
+  for (; v + G * U <= p.v1; v += G * U) {
     uint4 w[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (v + k * G < p.v1) w[k] = vecs[v + k * G];
+    for (int k = 0; k < U; ++k) w[k] = vecs[v + k * G];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (v + k * G >= p.v1) continue;
-      float f[VEC];
-      L::unpack(w[k], f);
+    for (int k = 0; k < U; ++k) grad_vector<T, ENT>(out + (v + k * G) * VEC, w[k], c, g, same_phase);
+  }
+  for (; v + tid < p.v1; v += G) grad_vector<T, ENT>(out + v * VEC, vecs[v], c, g, same_phase);
+}
+template <typename T>
+__device__ __forceinline__ void zero_vector(T* out, bool same_phase) {
+  if (same_phase) {
+    *reinterpret_cast<uint4*>(out) = make_uint4(0u, 0u, 0u, 0u);
+  } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = grad_at<ENT>(f[i], c, g);
-      T* out = dx + p.vec_base + (v + k * G) * VEC;
-      if (same_phase) {
-        *reinterpret_cast<uint4*>(out) = L::pack(f);
-      } else {  // logits and gradient start at different offsets within 16 bytes
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) out[i] = L::down(f[i]);
-      }
-    }
+    for (int i = 0; i < LogitType<T>::VEC; ++i) out[i] = LogitType<T>::down(0.0f);
   }
 }
 template <typename T, int G>
@@ -669,15 +760,7 @@ __device__ __forceinline__ void zero_grad(const RowPart<T>& p, T* dx, bool same_
   const T zero = LogitType<T>::down(0.0f);
   if (tid < p.head) dx[tid] = zero;
   if (tid < p.tail) dx[p.tail_base + tid] = zero;
-  for (int v = p.v0 + tid; v < p.v1; v += G) {
-    T* out = dx + p.vec_base + v * VEC;
-    if (same_phase) {
-      *reinterpret_cast<uint4*>(out) = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = zero;
-    }
-  }
+  for (int v = p.v0 + tid; v < p.v1; v += G) zero_vector<T>(dx + p.vec_base + v * VEC, same_phase);
 }
 // Entries (index, weight) added to the gradient: each is written once, as the rounding of dense value plus the sum of
 // all weights with its index, in list order (the same index may come several times).  idx < 0 marks no entry.  Runs
