@@ -437,8 +437,7 @@ class Backend:
         self._bind_stream()
         check(self.lib.mtb200_token_log_probs(
             self._h, code, rows, vocab, logits.data_ptr(), ld, _ptr(tokens), I32 if tokens is None else _DTYPES[tokens.dtype],
-            ignore_index is not None, ignore_index or 0, temperature, top, _ptr(out.log_probs), _ptr(out.entropy),
-            _ptr(out.top_log_probs), _ptr(out.top_indices), _ptr(out.stats)))
+            ignore_index is not None, ignore_index or 0, temperature, top, *(None if t is None else t.data_ptr() for t in out)))
         self.launches += 1
         return out
 

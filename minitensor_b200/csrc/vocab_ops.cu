@@ -57,6 +57,27 @@ struct Block {
   static __device__ __forceinline__ int part(int parts) { return G == 32 ? 0 : blockIdx.x % static_cast<unsigned>(parts); }
 };
 
+// The same for kernels whose blocks do not meet: `whole` rows with a block each, then the others in `parts` parts.
+template <int G>
+struct Cut {
+  long long row;  // -1: nothing to do
+  int part, parts;
+  __device__ __forceinline__ Cut(int rows, int whole, int cut_parts) {
+    const unsigned unit = G == 32 ? blockIdx.x * Block<G>::ROWS + Block<G>::slot() : blockIdx.x;
+    if (unit < static_cast<unsigned>(whole)) {
+      row = unit;
+      part = 0;
+      parts = 1;
+    } else {
+      const unsigned more = unit - whole;
+      row = static_cast<long long>(whole) + more / static_cast<unsigned>(cut_parts);
+      part = more % static_cast<unsigned>(cut_parts);
+      parts = cut_parts;
+      if (row >= rows) row = -1;
+    }
+  }
+};
+
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.442695040888963407f;
 
@@ -173,7 +194,7 @@ struct ScoreGradArgs {
   const void* logits;
   void* dlogits;
   long long ld;
-  int rows, vocab, top, parts, same_phase;
+  int rows, vocab, top, parts, whole, same_phase;
   IndexArray tokens;
   int has_ignore;
   long long ignore;
@@ -185,19 +206,20 @@ struct ScoreGradArgs {
 
 // dx = (1/T) [ sum of weights at given indices - p (sum of all weights) - g_H p (log p + H) ], one read, one write.
 template <typename T, int G, bool ENT>
-static __global__ void __launch_bounds__(Block<G>::THREADS) token_scores_grad_kernel(ScoreGradArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) token_scores_grad_kernel(ScoreGradArgs a) {
   __shared__ int all_idx[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
   __shared__ float all_weight[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
   __shared__ float fold[Group<G>::WARPS];
   int* idx = all_idx[Block<G>::slot()];
   float* weight = all_weight[Block<G>::slot()];
-  const int part = Block<G>::part(a.parts);
-  const long long r = Block<G>::row(a.rows, a.parts);
+  const Cut<G> cut(a.rows, a.whole, a.parts);
+  const int part = cut.part;
+  const long long r = cut.row;
   const int tid = Group<G>::rank();
   if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
-  const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
+  const RowPart<T> p = row_part(row, a.vocab, part, cut.parts);
   const long long token = a.tokens.p ? a.tokens.at(r) : -1;
   if (a.tokens.p && a.has_ignore && token == a.ignore) {
     zero_grad<T, G>(p, dx, a.same_phase);
@@ -243,7 +265,7 @@ struct DistillArgs {
   const void* logits;
   void* dlogits;           // forward: nullptr = loss only
   long long ld;
-  int rows, vocab, top, parts, same_phase;
+  int rows, vocab, top, parts, whole, same_phase;
   IndexArray index;
   RealArray value;
   float inv_t, c, t;
@@ -467,6 +489,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
         if (idx[k] == index && k != at) atomicOr(&twice[at], k < at ? 2 : 1);
   }
   __syncthreads();
+  if (a.parts > 1) cluster_arrive_relaxed();  // this block has received what it waits for
   const float4 info = row_sm;
   RowGrad g;
   g.base = info.x == -INFINITY ? 0.0f : info.x;
@@ -503,21 +526,23 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
       a.stats[2 * r + 1] = info.y;
     }
   }
+  if (a.parts > 1) cluster_wait();  // no block leaves while another may still send to it
 }
 
 template <typename T, int G>
-static __global__ void __launch_bounds__(Block<G>::THREADS) distill_grad_kernel(DistillArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) distill_grad_kernel(DistillArgs a) {
   __shared__ int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float fold[Group<G>::WARPS];
   int* idx = all_idx[Block<G>::slot()];
   float* q = all_q[Block<G>::slot()];
-  const int part = Block<G>::part(a.parts);
-  const long long r = Block<G>::row(a.rows, a.parts);
+  const Cut<G> cut(a.rows, a.whole, a.parts);
+  const int part = cut.part;
+  const long long r = cut.row;
   if (r < 0) return;
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
-  const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
+  const RowPart<T> p = row_part(row, a.vocab, part, cut.parts);
   float ln_sq;
   if (!load_teacher<G>(a, r, part == 0, idx, q, nullptr, fold, &ln_sq)) {
     zero_grad<T, G>(p, dx, a.same_phase);
@@ -580,10 +605,9 @@ static int32_t check_index(const char* what, int32_t dtype) {
   return MTB200_OK;
 }
 
-// One cluster of `parts` blocks per row, or with G = 32 a warp per row.  Kernels whose blocks do not meet take a plain
-// grid (`meet` false).
+// One cluster of `parts` blocks per row, or with G = 32 a warp per row.
 template <int G, typename Args>
-static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, bool meet, size_t smem = 0) {
+static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, size_t smem = 0) {
   if (smem > 48 * 1024)
     if (int32_t rc = grant_dynamic_smem(h, kernel, int(smem))) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -596,7 +620,7 @@ static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, b
   attr[0].val.clusterDim.x = unsigned(a.parts);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = meet && a.parts > 1 ? 1 : 0;
+  cfg.numAttrs = a.parts > 1 ? 1 : 0;
   MTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return MTB200_OK;
 }
@@ -630,29 +654,56 @@ static int32_t launch_scores(mtb200_ctx* h, const ScoreArgs& a) {
   if (a.top) smem = sizeof(TopScratch<G>) * Block<G>::ROWS + (a.parts > 1 ? sizeof(unsigned long long) * a.parts * a.top : 0);
   return launch_rows<G>(h, a.top ? (a.entropy ? token_scores_kernel<T, G, true, true> : token_scores_kernel<T, G, true, false>)
                                  : (a.entropy ? token_scores_kernel<T, G, false, true> : token_scores_kernel<T, G, false, false>),
-                        a, true, smem);
+                        a, smem);
+}
+// The gradient kernels' blocks do not meet, so that rows can be cut unevenly: `whole` rows go to a block each, as many as
+// make the same number for every SM, and the rows that are left are cut into the number of parts that spreads them best.
+// 601 x 32003 f32 on 148 SMs, four rows for each and nine over in 16 parts: 31.3 us, 35.3 us with a block for each of the
+// nine.  (Cutting all rows costs more than it spreads: 4096 x 128256 bf16 take 314 us whole and 366 us in parts of 64 KB.)
+static void cut_rows(const mtb200_ctx* h, int rows, int64_t row_bytes, int* whole, int* parts) {
+  const bool few = rows < 2 * h->sm_count;
+  const int left = few ? rows : rows % h->sm_count;
+  *whole = rows - left;
+  *parts = 1;
+  double best = 1e30;
+  for (int n = few && rows <= h->sm_count ? 2 : 1; n <= 16 && (n == 1 || row_bytes / n >= PART_BYTES); ++n) {
+    const double rounds = double((int64_t(left) * n + h->sm_count - 1) / h->sm_count) / n;
+    if (rounds < 0.95 * best) {  // worth the further blocks
+      best = rounds;
+      *parts = n;
+    }
+  }
+}
+template <int G, typename Args>
+static int32_t launch_cut(mtb200_ctx* h, void (*kernel)(Args), Args a, size_t row_bytes) {
+  a.whole = a.rows;
+  a.parts = 1;
+  if (G == 512) cut_rows(h, a.rows, int64_t(row_bytes), &a.whole, &a.parts);
+  const int64_t units = a.whole + int64_t(a.rows - a.whole) * a.parts;
+  kernel<<<unsigned((units + Block<G>::ROWS - 1) / Block<G>::ROWS), Block<G>::THREADS, 0, h->stream>>>(a);
+  MTB_CUDA(cudaGetLastError());
+  return MTB200_OK;
 }
 template <typename T, int G>
 static int32_t launch_score_grad(mtb200_ctx* h, const ScoreGradArgs& a) {
-  return launch_rows<G>(h, a.d_entropy ? token_scores_grad_kernel<T, G, true> : token_scores_grad_kernel<T, G, false>, a, false);
+  return launch_cut<G>(h, a.d_entropy ? token_scores_grad_kernel<T, G, true> : token_scores_grad_kernel<T, G, false>, a,
+                       a.vocab * sizeof(T));
 }
-#ifndef DMB
-#define DMB 32
-#endif
-#ifndef DPB
-#define DPB 32768
-#endif
+// Parts of a row for the step that looks at it twice: the rows in flight, three blocks of 512 threads on an SM, have to
+// stay in L2 beside the gradients that are written.  4096 x 128256 bf16, 114 MB of rows in flight without a cut: 435 us in 2
+// parts (57 MB), 518 in 1, 538 in 4, whose blocks do too little between their meetings.
+constexpr int64_t L2_ROWS_BYTES = int64_t(64) << 20;
 template <typename T, int G>
 static int32_t launch_distill(mtb200_ctx* h, const DistillArgs& a) {
   if constexpr (G == 512)
     if (a.row_loss && a.dlogits && a.top <= CLUSTER_TEACHER) {
       DistillArgs c = a;
       const int64_t row_bytes = int64_t(a.vocab) * sizeof(T);
-      while (c.parts < MAX_PARTS && 3 * h->sm_count / c.parts * row_bytes > (DMB << 20) && row_bytes / (c.parts * 2) >= DPB) c.parts *= 2;
-      return launch_rows<G>(h, distill_cluster_kernel<T>, c, true);
+      while (c.parts < MAX_PARTS && 3 * h->sm_count / c.parts * row_bytes > L2_ROWS_BYTES) c.parts *= 2;
+      return launch_rows<G>(h, distill_cluster_kernel<T>, c);
     }
-  if (!a.row_loss) return launch_rows<G>(h, distill_grad_kernel<T, G>, a, false);
-  return launch_rows<G>(h, a.dlogits ? distill_kernel<T, G, true> : distill_kernel<T, G, false>, a, true);
+  if (!a.row_loss) return launch_cut<G>(h, distill_grad_kernel<T, G>, a, a.vocab * sizeof(T));
+  return launch_rows<G>(h, a.dlogits ? distill_kernel<T, G, true> : distill_kernel<T, G, false>, a);
 }
 // f(element type, group size as a compile-time number)
 template <int G>

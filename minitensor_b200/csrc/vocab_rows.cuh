@@ -30,18 +30,6 @@ __device__ __forceinline__ float ex2_ftz(float x) {
   return y;
 }
 
-// 16 bytes from global to shared memory, both aligned, on the thread's own account: a group is what was asked for up to a
-// commit, and wait<N> returns when all groups but the last N have arrived, for the thread that asked.
-__device__ __forceinline__ void copy_async16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
-               : "memory");
-}
-__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Four words into the shared memory of block `rank` of the cluster, at the place that `to` has in this block; they count on
 // the barrier of that block at the place of `bar`.
 __device__ __forceinline__ void send_async(const void* to, const unsigned long long* bar, int rank, float4 v) {
@@ -52,6 +40,10 @@ __device__ __forceinline__ void send_async(const void* to, const unsigned long l
       "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w))
       : "memory");
 }
+
+// Cluster barrier that orders no memory operations, in two halves.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // Two f32 operations per instruction, each rounded as its scalar form.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -246,9 +238,9 @@ __device__ __forceinline__ bool owns(const RowPart<T>& p, int j) {
 }
 
 // ------------------------------------------------------------------ order of the selection
-// Larger logit first, ties to the lower index, -0 = +0, NaN ranks with -inf.  A candidate is
-// one 64-bit word, the order-preserving image of the logit above the complement of the index; larger is better, no
-// two are equal, and 0 is no candidate.
+// Larger logit first, ties to the lower index, -0 = +0, NaN ranks with -inf.  A candidate is one 64-bit word, the
+// order-preserving image of the logit above the complement of the index; larger is better, no two are equal, and 0 is no
+// candidate.
 __device__ __forceinline__ uint32_t rank_key(float x) {
   x = isnan(x) ? -INFINITY : x + 0.0f;
   const uint32_t b = __float_as_uint(x);
@@ -362,6 +354,7 @@ __device__ __forceinline__ void add_vector(float2& s, float2& u, const uint4& w,
   }
 }
 
+// The thread's unit, reduced.  All threads of a warp call it together.
 template <typename T, int G, bool ENT, bool TOP>
 __device__ __forceinline__ UnitStat unit_stats(const RowPart<T>& p, float c, uint16_t (*slots)[G]) {
   using L = LogitType<T>;
