@@ -629,28 +629,33 @@ static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, s
 struct RowPlan {
   int group, parts;
 };
-// A warp per row up to 8 KB (65536 x 1000 f32: 57 us against 460 us with a block of 512 per row), 128 threads up to 32 KB,
-// else blocks of 512.  Where whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long
-// as the parts still find room side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us
-// in 8, which run in two waves.
-constexpr int64_t WARP_BYTES = 8192, MID_BYTES = 32768, PART_BYTES = 8192;
-static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, int64_t warp_top, int64_t mid_top, int64_t top) {
-  if (row_bytes <= WARP_BYTES && top <= warp_top && rows > h->sm_count) return {32, 1};
-  if (row_bytes <= MID_BYTES && top <= mid_top) return {128, 1};
+// A warp per row up to 8 KB (65536 x 1000 f32: 60 us against 460 us with a block of 512 per row), 128 threads up to 32 KB, or
+// 64 KB with the selection, whose steps other rows have to hide (4096 x 16000 f32 with 20: 63 us against 100), else blocks of
+// 512.  Many alternatives need many units to choose from: beyond WARP_TOP the warp, beyond MID_TOP the 128 threads are
+// the slower (8192 x 1000 f16 with 32: 99 us by warps and 64 us by blocks; 4096 x 4000 f32 with 100: 214 and 108 us).  Where
+// whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long as the parts still find room
+// side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us in 8, which run in two waves.
+constexpr int64_t WARP_BYTES = 8192, MID_BYTES = 32768, MID_BYTES_TOP = 65536, PART_BYTES = 8192;
+constexpr int WARP_TOP = 20, MID_TOP = 64;
+static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, bool warp, int64_t mid_bytes) {
+  if (row_bytes <= WARP_BYTES && warp && rows > h->sm_count) return {32, 1};
+  if (row_bytes <= mid_bytes) return {128, 1};
   int parts = 1;
   while (parts < MAX_PARTS && rows * parts <= h->sm_count && row_bytes / (2 * parts) >= PART_BYTES) parts *= 2;
   return {512, parts};
 }
 
-// With the selection on rows of 16-bit logits, four blocks of 256 threads on an SM instead of two of 512: a block that selects
-// leaves three that stream.  4096 x 128256 bf16 and their best 20: 206 us against 239; f32, whose rows take twice the
-// time to stream, gains nothing (247 us against 234 on 2048 x 151936 with 64), nor do fewer rows than blocks, and from some
-// 64 on the candidates are too many for 256 threads.
+// With the selection on many rows, four blocks of 256 threads on an SM instead of two of 512: a block that selects leaves
+// three that stream.  4096 x 128256 bf16 and their best 20: 206 us against 239; 4096 x 60000 f32 180 against 213.  Rows that
+// take longer to stream gain nothing (2048 x 151936 f32 with 64: 247 us against 234), nor do fewer rows than blocks, and
+// from some 64 on the candidates are too many for 256 threads.
+constexpr int64_t QUAD_BYTES = 256 << 10;
 template <typename T, int G>
 static int32_t launch_scores(mtb200_ctx* h, const ScoreArgs& a) {
   size_t smem = 0;
   if constexpr (G == 512)
-    if (a.top && a.top <= 64 && sizeof(T) == 2 && a.rows > 2 * h->sm_count) return launch_scores<T, 256>(h, a);
+    if (a.top && a.top <= MID_TOP && (sizeof(T) == 2 || a.vocab * int64_t(sizeof(T)) <= QUAD_BYTES) && a.rows > 2 * h->sm_count)
+      return launch_scores<T, 256>(h, a);
   if (a.top) smem = sizeof(TopScratch<G>) * Block<G>::ROWS + (a.parts > 1 ? sizeof(unsigned long long) * a.parts * a.top : 0);
   return launch_rows<G>(h, a.top ? (a.entropy ? token_scores_kernel<T, G, true, true> : token_scores_kernel<T, G, true, false>)
                                  : (a.entropy ? token_scores_kernel<T, G, false, true> : token_scores_kernel<T, G, false, false>),
@@ -758,7 +763,8 @@ int32_t mtb200_token_log_probs(mtb200_handle h, int32_t dtype, int64_t rows, int
   a.inv_t = float(1.0 / temperature); a.c = float(1.4426950408889634 / temperature);
   a.log_probs = tokens ? log_probs : nullptr; a.entropy = entropy; a.top_log_probs = top_log_probs;
   a.top_indices = top_indices; a.stats = stats; a.bad_label = h->status + 1;
-  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), TopScratch<32>::MOST, TopScratch<128>::MOST, top);
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), top <= WARP_TOP,
+                                 top == 0 ? MID_BYTES : top <= MID_TOP ? MID_BYTES_TOP : 0);
   a.parts = plan.parts;
   return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_scores<decltype(element), group_of(tag)>(h, a); });
 }
@@ -787,7 +793,7 @@ int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows,
   a.stats = stats; a.entropy = entropy; a.d_log_probs = d_log_probs; a.d_entropy = d_entropy; a.d_top = d_top;
   a.top_indices = top_indices; a.bad_label = h->status + 1;
   a.same_phase = same_phase(logits, dlogits);
-  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), VOCAB_TOP_MAX, VOCAB_TOP_MAX, top);
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), true, MID_BYTES);
   a.parts = plan.parts;
   return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_score_grad<decltype(element), group_of(tag)>(h, a); });
 }
@@ -816,7 +822,7 @@ static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, in
   a->scale = float(temperature * (reduction == MTB200_REDUCE_MEAN && rows ? 1.0 / double(rows) : 1.0) * double(upstream));
   a->upstream_rows = upstream_rows; a->status = h->status; a->bad_label = h->status + 1;
   a->same_phase = same_phase(logits, dlogits);
-  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), TEACHER_WARP_MAX, VOCAB_TEACHER_MAX, top);
+  const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), top <= TEACHER_WARP_MAX, MID_BYTES);
   a->parts = plan.parts;
   *group = plan.group;
   return MTB200_OK;

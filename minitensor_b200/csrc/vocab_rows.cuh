@@ -494,13 +494,14 @@ __device__ __forceinline__ void for_each_rank(const unsigned long long* list, in
     if (i < n && sub == 0) f(i, above);
   }
 }
-// The best `count` of pool[0, n) into best[0, count) in order: by counting, or where the block's threads can take one
-// candidate each and counting would take longer (n^2 / 128 steps of a warp against 45 exchanges), by a bitonic sort,
-// within a warp by shuffles and across warps through the pool itself.  Every thread of the group takes part.
+// The best `count` of pool[0, n) into best[0, count) in order, by counting, or by a bitonic sort where counting would take
+// longer (n^2 / 128 steps of a warp).  With a candidate for each of 512 threads the sort goes by shuffles within a warp
+// and through the pool across warps; with more candidates, which few units of many alternatives or ties bring about, in
+// the pool (`room` words, those behind n are free).  Every thread of the group takes part.
 template <int G>
-__device__ __forceinline__ void rank_pool(unsigned long long* pool, int n, int count, unsigned long long* best) {
+__device__ __forceinline__ void rank_pool(unsigned long long* pool, int n, int room, int count, unsigned long long* best) {
+  const int tid = Group<G>::rank();
   if (G == 512 && n > 160 && n <= G) {
-    const int tid = threadIdx.x;
     unsigned long long w = tid < n ? pool[tid] : 0ull;
     for (int size = 2; size <= G; size <<= 1) {
       const bool down = (tid & size) == 0 || size == G;
@@ -518,6 +519,25 @@ __device__ __forceinline__ void rank_pool(unsigned long long* pool, int n, int c
       }
     }
     if (tid < count) best[tid] = w;
+    return;
+  }
+  const int all = n > 1 ? 1 << (32 - __clz(n - 1)) : 1;
+  if (n > 512 && all <= room) {
+    for (int i = n + tid; i < all; i += G) pool[i] = 0ull;
+    Group<G>::sync();
+    for (int size = 2; size <= all; size <<= 1)
+      for (int o = size >> 1; o; o >>= 1) {
+        for (int i = tid; i < all / 2; i += G) {
+          const int a = 2 * i - (i & (o - 1)), b = a + o;  // i-th pair that is o apart
+          const unsigned long long x = pool[a], y = pool[b];
+          if ((x < y) == ((a & size) == 0)) {
+            pool[a] = y;
+            pool[b] = x;
+          }
+        }
+        Group<G>::sync();
+      }
+    for (int i = tid; i < count; i += G) best[i] = pool[i];
     return;
   }
   for_each_rank<G>(pool, n, [&](int i, int above) {
@@ -667,7 +687,7 @@ __device__ void select_top(const RowPart<T>& p, int top, float unit_max, int whe
       n = ts.pool_count;
       Group<G>::sync();  // every thread has the same n before anyone offers more
       if (n > CAPACITY - AT_ONCE * VEC && base + AT_ONCE < total) {
-        rank_pool<G>(ts.pool, n, top, ts.best);
+        rank_pool<G>(ts.pool, n, CAPACITY, top, ts.best);
         Group<G>::sync();
         for (int j = tid; j < top; j += G) ts.pool[j] = ts.best[j];
         if (tid == 0) ts.pool_count = top;
@@ -676,7 +696,7 @@ __device__ void select_top(const RowPart<T>& p, int top, float unit_max, int whe
       }
     }
   }
-  rank_pool<G>(ts.pool, n, top, ts.best);
+  rank_pool<G>(ts.pool, n, CAPACITY, top, ts.best);
   Group<G>::sync();
 }
 
