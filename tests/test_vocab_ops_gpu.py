@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # (rows, vocabulary, extra columns in memory): one token and one class, odd sizes, parts of a vector, several blocks a row
 SHAPES = [(1, 1, 0), (1, 2, 1), (3, 7, 0), (5, 8, 8), (9, 127, 3), (4, 1000, 0), (33, 4099, 13), (2, 32003, 61), (301, 6007, 1),
-          (700, 515, 0), (1, 200001, 7), (320, 20001, 2)]
+          (700, 515, 0), (1, 200001, 7), (320, 20001, 2), (300, 40009, 3), (298, 70001, 0)]
 
 
 def logits_for(rows, vocab, pad, dtype, seed, spread=2.5):
@@ -543,6 +543,57 @@ def test_offsets_beyond_32_bits(be):
     check_score_grad(be, x, tokens, 1.0, 9)
     idx, val = teacher_for(rows, vocab, 9, 6)
     check_distill(be, x, idx, val, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(2, 2500001), (200, 600011)])
+def test_very_long_rows(be, dtype, rows, vocab):
+    """Rows of many rounds per thread: the selection's spans cover several rounds each."""
+    x = logits_for(rows, vocab, 0, dtype, vocab)
+    x[0, ::2] = -math.inf
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) | 1
+    tokens = tokens.clamp(max=vocab - 1)
+    for top in (20, 256):
+        got = be.token_log_probs(x, tokens, top=top, entropy=True)
+        be.sync()
+        for i in range(0, rows, 40):   # some rows at a time: the 64-bit definition takes 8 bytes an element and more
+            part = slice(i, min(rows, i + 2))
+            p, lp = ref.softmax64(x[part], 1.0)
+            want = lp.gather(1, tokens[part, None])[:, 0]
+            close(got.log_probs[part], want, ref.log_prob_tolerance(want, vocab))
+            h = ref.entropy64(p, lp)
+            close(got.entropy[part], h, ref.entropy_tolerance(h, vocab))
+            assert torch.equal(got.top_indices[part].long(), ref.order64(x[part], top))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(200, 257), (200, 1000), (170, 2048), (300, 33000)])
+def test_nearly_all_entries_wanted(be, dtype, rows, vocab):
+    """Many alternatives of short rows: more wanted than there are threads' shares, and candidates by the thousand."""
+    x = logits_for(rows, vocab, 0, dtype, 17)
+    x[3] = 1.0
+    x[4, 5:] = -math.inf
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    for top in (21, 65, 128, 129, 256):
+        check_scores(be, x, tokens, 1.0, top)
+
+
+def test_two_backends_and_backward_after_other_calls(be):
+    """Statistics belong to the caller: another handle, and other calls in between, change nothing."""
+    from minitensor_b200.backend import Backend
+    other = Backend(0)
+    x, y = logits_for(30, 9001, 0, torch.float32, 1), logits_for(30, 9001, 0, torch.float32, 2)
+    tokens = torch.arange(30, device="cuda")
+    fwd = be.token_log_probs(x, tokens, top=5, entropy=True)
+    d = torch.ones(30, device="cuda")
+    first = be.token_log_probs_bwd(x, tokens, fwd.stats, d_log_probs=d, entropy=fwd.entropy, d_entropy=d)
+    other.token_log_probs(y, tokens, top=5, entropy=True)
+    be.token_log_probs(y, tokens, top=7)
+    second = other.token_log_probs_bwd(x, tokens, fwd.stats, d_log_probs=d, entropy=fwd.entropy, d_entropy=d)
+    other.sync()
+    be.sync()
+    assert torch.equal(first, second)
+    other.close()
 
 
 def test_refusals_on_the_device(be):
