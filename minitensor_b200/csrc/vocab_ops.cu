@@ -392,10 +392,10 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
 }
 
 // Loss and gradient of long rows: a cluster per row, so that the rows in flight stay in L2 between the two looks at them
-// (2048 x 128256 f32 with a block per row: 493 us, as long as two reads and a write from HBM take).  A block's chain of steps
-// is short: its logits are asked for first; what a row needs once is done by one warp, what its entries need by the warps
-// that have entries (from the second on: thread 32 + e has entry e); and the parts exchange their statistics by messages
-// instead of a cluster barrier, which would wait for all memory operations under way.
+// (2048 x 128256 f32: 398 us; with a block per row 493 us, as long as two reads and a write from HBM take).  Two
+// exponentials per element and the meetings between the two looks bound it: what a row needs once is done by one warp,
+// what its entries need by the warps that have entries (from the second on: thread 32 + e has entry e), and the parts
+// exchange their statistics by messages instead of a cluster barrier, which would wait for all memory operations under way.
 constexpr int CLUSTER_TEACHER = 480;  // entries
 template <typename T>
 static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillArgs a) {

@@ -42,8 +42,8 @@ __device__ __forceinline__ void send_async(const void* to, const unsigned long l
 }
 
 // Cluster barrier that orders no memory operations, in two halves.
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 
 // Two f32 operations per instruction, each rounded as its scalar form.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
