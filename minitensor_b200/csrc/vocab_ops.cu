@@ -120,10 +120,10 @@ struct RowOut {
 };
 
 // A cluster of `parts` blocks per row (one block when there are rows enough, a warp for short rows).  One pass over the
-// logits: HBM-bound.  Registers decide how many blocks share an SM: three of 512 threads without the selection; with it
-// 1024 threads, whose 64 registers keep the four loads of a round together.
+// logits: HBM-bound.  Registers decide how many blocks share an SM: 1536 threads of 40 registers without the selection; with
+// it 1024, whose 64 registers keep the four loads of a round together.
 template <typename T, int G, bool TOP, bool ENT>
-static __global__ void __launch_bounds__(Block<G>::THREADS, TOP ? (G >= 256 ? 1024 / G : 1) : (G == 512 ? 3 : 1)) token_scores_kernel(ScoreArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, (TOP ? 1024 : 1536) / Block<G>::THREADS) token_scores_kernel(ScoreArgs a) {
   using L = LogitType<T>;
   extern __shared__ __align__(16) unsigned char dynamic_smem[];
   __shared__ RowStat sm[Group<G>::WARPS + 1], parts_st[MAX_PARTS];
@@ -207,7 +207,7 @@ struct ScoreGradArgs {
 // dx = (1/T) [ sum of weights at given indices - p (sum of all weights) - g_H p (log p + H) ], one read, one write.
 template <typename T, int G, bool ENT>
 static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) token_scores_grad_kernel(ScoreGradArgs a) {
-  __shared__ int all_idx[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
+  __shared__ __align__(16) int all_idx[Block<G>::ROWS][VOCAB_TOP_MAX + 4];
   __shared__ float all_weight[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
   __shared__ float fold[Group<G>::WARPS];
   int* idx = all_idx[Block<G>::slot()];
@@ -247,6 +247,7 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) to
     weight[e] = w * a.inv_t;
     sum += w;
   }
+  fill_list<G>(idx, n);
   sum = group_fold<G, false>(sum, fold);
   RowGrad g;
   const float m = a.stats[2 * r];
@@ -297,6 +298,7 @@ __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, 
     top = fmaxf(top, q[e]);
     any = any || (in && q[e] != -INFINITY);  // NaN counts: it has to reach the result
   }
+  fill_list<G>(idx, a.top);  // TEACHER_ROOM is a multiple of four
   any = G == 32 ? __any_sync(0xffffffffu, any) : Group<G>::count(any) > 0;
   if (!any) return false;
   top = group_fold<G, true>(top, fold);
@@ -323,7 +325,7 @@ template <typename T, int G, bool GRAD>
 static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(DistillArgs a) {
   using L = LogitType<T>;
   __shared__ RowStat sm[Group<G>::WARPS + 1], parts_st[MAX_PARTS];
-  __shared__ int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ __align__(16) int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>], all_dv[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float fold[Group<G>::WARPS];
   int* idx = all_idx[Block<G>::slot()];
@@ -531,7 +533,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
 
 template <typename T, int G>
 static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) distill_grad_kernel(DistillArgs a) {
-  __shared__ int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
+  __shared__ __align__(16) int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float fold[Group<G>::WARPS];
   int* idx = all_idx[Block<G>::slot()];
@@ -629,16 +631,17 @@ static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, s
 struct RowPlan {
   int group, parts;
 };
-// A warp per row up to 8 KB (65536 x 1000 f32: 60 us against 460 us with a block of 512 per row), 128 threads up to 32 KB, or
-// 64 KB with the selection, whose steps other rows have to hide (4096 x 16000 f32 with 20: 63 us against 100), else blocks of
-// 512.  Many alternatives need many units to choose from: beyond WARP_TOP the warp, beyond MID_TOP the 128 threads are
+// A warp per row up to 8 KB where the rows are many (65536 x 1000 f32: 60 us against 460 us with a block of 512 per row; 300 x
+// 4000 f16 with 20 alternatives take 16.0 us by warps and 6.4 us by 128 threads, 2000 rows 20.8 and 15.7 us, 2000 x 1000 f32
+// 11.5 and 13.4 us), 128 threads up to 32 KB, or 64 KB with the selection, whose steps other rows have to hide (4096 x 16000
+// f32 with 20: 63 us against 100), else blocks of 512.  Many alternatives need many units to choose from: beyond WARP_TOP the warp, beyond MID_TOP the 128 threads are
 // the slower (8192 x 1000 f16 with 32: 99 us by warps and 64 us by blocks; 4096 x 4000 f32 with 100: 214 and 108 us).  Where
 // whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long as the parts still find room
 // side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us in 8, which run in two waves.
 constexpr int64_t WARP_BYTES = 8192, MID_BYTES = 32768, MID_BYTES_TOP = 65536, PART_BYTES = 8192;
 constexpr int WARP_TOP = 20, MID_TOP = 64;
 static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, bool warp, int64_t mid_bytes) {
-  if (row_bytes <= WARP_BYTES && warp && rows > h->sm_count) return {32, 1};
+  if (row_bytes <= WARP_BYTES && warp && rows > 8 * h->sm_count) return {32, 1};
   if (row_bytes <= mid_bytes) return {128, 1};
   int parts = 1;
   while (parts < MAX_PARTS && rows * parts <= h->sm_count && row_bytes / (2 * parts) >= PART_BYTES) parts *= 2;

@@ -776,23 +776,39 @@ __device__ __forceinline__ void zero_grad(const RowPart<T>& p, T* dx, bool same_
   for (int v = p.v0 + tid; v < p.v1; v += G) zero_vector<T>(dx + p.vec_base + v * VEC, same_phase);
 }
 // Entries (index, weight) added to the gradient: each is written once, as the rounding of dense value plus the sum of
-// all weights with its index, in list order (the same index may come several times).  idx < 0 marks no entry.  Runs
-// after the group barrier that follows dense_grad.
+// all weights with its index, in list order (the same index may come several times).  idx < 0 marks no entry; the list is
+// 16-byte aligned and read four at a time, up to three places beyond n (fill_list).  Runs after the group barrier that
+// follows dense_grad.
+template <int G>
+__device__ __forceinline__ void fill_list(int* idx, int n) {  // before a group barrier
+  if (Group<G>::rank() < (-n & 3)) idx[n + Group<G>::rank()] = -1;
+}
 template <typename T, int G, bool ENT>
 __device__ __forceinline__ void sparse_fix(const RowPart<T>& p, T* dx, float c, const RowGrad& g, const int* idx,
                                            const float* weight, int n) {
   using L = LogitType<T>;
+  const int4* list = reinterpret_cast<const int4*>(idx);
   for (int e = Group<G>::rank(); e < n; e += G) {
     const int j = idx[e];
     if (j < 0 || !owns(p, j)) continue;
-    float w = 0.0f;
-    bool leader = true;
-    for (int k = 0; k < n; ++k) {
-      if (idx[k] != j) continue;
-      leader = leader && k >= e;
-      w += weight[k];
+    int same = 0, first = INT_MAX;
+#pragma unroll 4
+    for (int k = 0; k < (n + 3) / 4; ++k) {
+      const int4 w = list[k];
+      const int hits = (w.x == j) | (w.y == j) << 1 | (w.z == j) << 2 | (w.w == j) << 3;
+      if (hits) {
+        same += __popc(hits);
+        first = min(first, 4 * k + __ffs(hits) - 1);
+      }
     }
-    if (leader) dx[j] = L::down(grad_at<ENT>(L::up(p.row[j]), c, g) + w);
+    if (first != e) continue;
+    float w = weight[e];
+    if (same > 1) {
+      w = 0.0f;
+      for (int k = 0; k < n; ++k)
+        if (idx[k] == j) w += weight[k];
+    }
+    dx[j] = L::down(grad_at<ENT>(L::up(p.row[j]), c, g) + w);
   }
 }
 

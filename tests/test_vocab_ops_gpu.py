@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # (rows, vocabulary, extra columns in memory): one token and one class, odd sizes, parts of a vector, several blocks a row
 SHAPES = [(1, 1, 0), (1, 2, 1), (3, 7, 0), (5, 8, 8), (9, 127, 3), (4, 1000, 0), (33, 4099, 13), (2, 32003, 61), (301, 6007, 1),
-          (700, 515, 0), (1, 200001, 7), (320, 20001, 2), (300, 40009, 3), (298, 70001, 0)]
+          (700, 515, 0), (1, 200001, 7), (320, 20001, 2), (300, 40009, 3), (298, 70001, 0), (1500, 515, 1)]
 
 
 def logits_for(rows, vocab, pad, dtype, seed, spread=2.5):
@@ -66,7 +66,7 @@ def test_scores_against_the_definition(be, dtype, rows, vocab, pad, top, tempera
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,vocab", [(6, 37), (6, 5003), (400, 5003), (6, 40009)])
+@pytest.mark.parametrize("rows,vocab", [(6, 37), (6, 5003), (400, 5003), (6, 40009), (1500, 333)])
 def test_masked_and_empty_rows(be, dtype, rows, vocab):
     x = logits_for(rows, vocab, 0, dtype, 5)
     lowest = torch.finfo(dtype).min
@@ -567,7 +567,7 @@ def test_very_long_rows(be, dtype, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,vocab", [(200, 257), (200, 1000), (170, 2048), (300, 33000)])
+@pytest.mark.parametrize("rows,vocab", [(200, 257), (200, 1000), (170, 2048), (300, 33000), (1300, 300)])
 def test_nearly_all_entries_wanted(be, dtype, rows, vocab):
     """Many alternatives of short rows: more wanted than there are threads' shares, and candidates by the thousand."""
     x = logits_for(rows, vocab, 0, dtype, 17)
