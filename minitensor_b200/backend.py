@@ -429,17 +429,26 @@ class Backend:
         if top < 0 or top > vocab:
             raise ValueError(f"{what}: top must be between 0 and the vocabulary's {vocab} entries, got {top}")
         dev, f32 = logits.device, torch.float32
-        out = TokenLogProbs(torch.empty(rows, dtype=f32, device=dev) if tokens is not None else None,
-                            torch.empty(rows, dtype=f32, device=dev) if entropy else None,
-                            torch.empty(rows, top, dtype=f32, device=dev) if top else None,
-                            torch.empty(rows, top, dtype=torch.int32, device=dev) if top else None,
-                            torch.empty(rows, 2, dtype=f32, device=dev))
+        log_probs = h = top_log_probs = top_indices = p_lp = p_h = p_tlp = p_ti = None
+        token_ptr, token_code = None, I32
+        if tokens is not None:
+            token_ptr, token_code = _ptr(tokens), _DTYPES[tokens.dtype]
+            log_probs = torch.empty(rows, dtype=f32, device=dev)
+            p_lp = log_probs.data_ptr()
+        if entropy:
+            h = torch.empty(rows, dtype=f32, device=dev)
+            p_h = h.data_ptr()
+        if top:
+            top_log_probs = torch.empty(rows, top, dtype=f32, device=dev)
+            top_indices = torch.empty(rows, top, dtype=torch.int32, device=dev)
+            p_tlp, p_ti = top_log_probs.data_ptr(), top_indices.data_ptr()
+        stats = torch.empty(rows, 2, dtype=f32, device=dev)
         self._bind_stream()
         check(self.lib.mtb200_token_log_probs(
-            self._h, code, rows, vocab, logits.data_ptr(), ld, _ptr(tokens), I32 if tokens is None else _DTYPES[tokens.dtype],
-            ignore_index is not None, ignore_index or 0, temperature, top, *(None if t is None else t.data_ptr() for t in out)))
+            self._h, code, rows, vocab, logits.data_ptr(), ld, token_ptr, token_code, ignore_index is not None,
+            ignore_index or 0, temperature, top, p_lp, p_h, p_tlp, p_ti, stats.data_ptr()))
         self.launches += 1
-        return out
+        return TokenLogProbs(log_probs, h, top_log_probs, top_indices, stats)
 
     def token_log_probs_bwd(self, logits: torch.Tensor, tokens: Optional[torch.Tensor], stats: torch.Tensor, *,
                             d_log_probs: Optional[torch.Tensor] = None, entropy: Optional[torch.Tensor] = None,
