@@ -368,11 +368,12 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
     for (int e = tid; e < a.top; e += G) {
       if (idx[e] < 0 || q[e] == 0.0f) continue;
       const float dx = none ? -INFINITY : L::up(row[idx[e]]) - st.m;
-      kl += q[e] * ((dv[e] - dx) * a.inv_t - (ln_sq - ln_s));
+      // T times the term, and T again on q: where T < 1, (dv - dx) / T or the sum without T may overflow
+      kl += a.t * q[e] * (dv[e] - dx - a.t * (ln_sq - ln_s));
     }
     kl = group_fold<G, false>(kl, fold);
     if (tid == 0) {
-      a.row_loss[r] = a.t * a.t * kl;
+      a.row_loss[r] = kl;
       if (a.stats) {
         a.stats[2 * r] = st.m;
         a.stats[2 * r + 1] = ln_s;
@@ -504,7 +505,8 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
   if (entry_warp && part == 0) {
     // log q - log p with the two maxima taken out first: nearly equal distributions lose nothing to the logarithms' size
     float kl = 0.0f;
-    if (mine >= 0 && q != 0.0f) kl = q * ((dv - (info.z != 0.0f ? -INFINITY : L::up(x_mine) - info.x)) * a.inv_t - (ln_sq - info.y));
+    // the factors T where distill_kernel has them
+    if (mine >= 0 && q != 0.0f) kl = a.t * q * (dv - (info.z != 0.0f ? -INFINITY : L::up(x_mine) - info.x) - a.t * (ln_sq - info.y));
 #pragma unroll
     for (int o = 16; o; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
     if (lane == 0) kl_sm[warp] = kl;
@@ -522,7 +524,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
   if (part == 0 && tid == 0) {
     float kl = 0.0f;
     for (int k = 1; k < WARPS && 32 * (k - 1) < a.top; ++k) kl += kl_sm[k];
-    a.row_loss[r] = a.t * a.t * kl;
+    a.row_loss[r] = kl;
     if (a.stats) {
       a.stats[2 * r] = info.x;
       a.stats[2 * r + 1] = info.y;

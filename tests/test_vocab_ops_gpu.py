@@ -321,6 +321,22 @@ def test_distillation_without_entries_and_with_the_most(be, dtype):
     check_distill(be, x, idx, val, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(3, 40), (2000, 40), (2, 50257), (700, 2003)])
+def test_distillation_of_the_lowest_logit_below_temperature_one(be, dtype, rows, vocab):
+    """The teacher wants an entry that holds the type's lowest value: (v - m) / T is beyond f32, T times it is not."""
+    x = logits_for(rows, vocab, 0, dtype, vocab)
+    idx, val = teacher_for(rows, vocab, 7, vocab)
+    x[0, idx[0, 2].long()] = torch.finfo(dtype).min
+    if rows > 2:
+        idx[2] = idx[2, 0].item()                              # all of a row's weight on that value
+        x[2, idx[2, 0].long()] = torch.finfo(dtype).min
+    check_distill(be, x, idx, val, 0.3)
+    loss, _ = be.distillation_loss(x, idx, val, temperature=0.3, reduction="none")
+    be.sync()
+    assert torch.isfinite(loss).all()
+
+
 def test_distillation_nan_teacher_and_bad_index(be):
     x = logits_for(4, 500, 0, torch.float32, 8)
     idx, val = teacher_for(4, 500, 6, 2)
