@@ -269,7 +269,7 @@ struct DistillArgs {
   int rows, vocab, top, parts, whole, same_phase;
   IndexArray index;
   RealArray value;
-  float inv_t, c, t;
+  float c, t;
   float scale;             // T * reduction factor * upstream: d loss / d logits = scale * weight_r * (Q p - q)
   const float* upstream_rows;
   float *row_loss, *stats;
@@ -823,7 +823,7 @@ static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, in
   a->logits = logits; a->dlogits = dlogits; a->ld = ld; a->rows = int(rows); a->vocab = int(vocab); a->top = int(top);
   a->index = {teacher_indices, index_dtype == MTB200_I64};
   a->value = {teacher_logits, teacher_dtype};
-  a->t = float(temperature); a->inv_t = float(1.0 / temperature); a->c = float(1.4426950408889634 / temperature);
+  a->t = float(temperature); a->c = float(1.4426950408889634 / temperature);
   a->scale = float(temperature * (reduction == MTB200_REDUCE_MEAN && rows ? 1.0 / double(rows) : 1.0) * double(upstream));
   a->upstream_rows = upstream_rows; a->status = h->status; a->bad_label = h->status + 1;
   a->same_phase = same_phase(logits, dlogits);
