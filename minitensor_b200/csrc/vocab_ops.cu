@@ -609,10 +609,14 @@ static int32_t check_index(const char* what, int32_t dtype) {
   return MTB200_OK;
 }
 
+// Dynamic shared memory that a kernel gets without asking.  The 48 KB of such a launch hold its static shared memory as well;
+// token_scores_kernel, the only kernel here with dynamic shared memory, has 304 bytes of it at most.
+constexpr size_t FREE_DYNAMIC_SMEM = 32 * 1024;
+
 // One cluster of `parts` blocks per row, or with G = 32 a warp per row.
 template <int G, typename Args>
 static int32_t launch_rows(mtb200_ctx* h, void (*kernel)(Args), const Args& a, size_t smem = 0) {
-  if (smem > 48 * 1024)
+  if (smem > FREE_DYNAMIC_SMEM)
     if (int32_t rc = grant_dynamic_smem(h, kernel, int(smem))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = smem;

@@ -642,3 +642,38 @@ def test_refusals_on_the_device(be):
     loss, grad = be.distillation_loss(x[:0], torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, 3, device="cuda"), reduction="sum")
     be.sync()
     assert loss.item() == 0.0 and grad.shape == (0, 50)
+
+
+_RISING_TOPS = """
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+import vocab_reference as ref
+from test_vocab_ops_gpu import check_scores, close, logits_for
+from minitensor_b200.backend import get_backend
+be = get_backend(0)
+for dtype in (torch.float32, torch.bfloat16, torch.float16):
+    x = logits_for(9, 128256 if dtype != torch.float32 else 50257, 0, dtype, 13)
+    tokens = torch.arange(9, device="cuda")
+    _, lp = ref.softmax64(x, 1.0)
+    for top in range(130, 144):
+        check_scores(be, x, tokens, 1.0, top)
+        got = be.token_log_probs(x, tokens, top=top)
+        be.sync()
+        order = ref.order64(x, top)
+        assert torch.equal(got.top_indices.long(), order)
+        want = lp.gather(1, order)
+        close(got.top_log_probs, want, ref.log_prob_tolerance(want, x.shape[1]))
+"""
+
+
+def test_more_alternatives_from_call_to_call_in_a_new_process():
+    """Few long rows are cut into eight parts, whose lists of alternatives lie in shared memory beside the scratch of the
+    selection: with rising `top` the sum passes the size that a launch may have without asking.  What a process has asked
+    for stays granted, so the calls come in a process of their own."""
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    script = _RISING_TOPS.format(root=ROOT, tests=os.path.join(ROOT, "tests"))
+    run = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert run.returncode == 0, run.stderr[-2000:]
