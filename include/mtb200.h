@@ -299,6 +299,15 @@ int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows,
                                    int64_t ignore_index, double temperature, const float* stats,
                                    const float* d_log_probs, const float* entropy, const float* d_entropy,
                                    int64_t top, const int32_t* top_indices, const float* d_top, void* dlogits);
+/* The _ex entries take a row stride of the gradient of its own (ld_grad >= vocab elements): logits that are a slice with far
+ * longer strides, such as the last position of every sequence, need no gradient of that size.  Where ld and ld_grad, and the
+ * two addresses, differ by multiples of 16 bytes, gradients are stored in whole vectors. */
+int32_t mtb200_token_log_probs_bwd_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits,
+                                      int64_t ld, const void* tokens, int32_t token_dtype, int32_t has_ignore,
+                                      int64_t ignore_index, double temperature, const float* stats,
+                                      const float* d_log_probs, const float* entropy, const float* d_entropy,
+                                      int64_t top, const int32_t* top_indices, const float* d_top, void* dlogits,
+                                      int64_t ld_grad);
 /* distill: Kullback-Leibler divergence of the student's p from a teacher known by `top` (0 .. 1024) entries per row,
  *   teacher_indices [rows][top] (int32 / int64) and teacher_logits [rows][top] (f32 / f16 / bf16; logits or log
  *   probabilities alike):  q = softmax(teacher_logits / T) over the entries whose index is not -1,
@@ -317,6 +326,15 @@ int32_t mtb200_distill_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t
                            int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
                            int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
                            const float* upstream_rows, const float* stats, void* dlogits);
+int32_t mtb200_distill_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                          int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                          int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                          const float* upstream_rows, float* row_loss, float* loss, float* stats, void* dlogits,
+                          int64_t ld_grad);
+int32_t mtb200_distill_bwd_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                              int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                              int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                              const float* upstream_rows, const float* stats, void* dlogits, int64_t ld_grad);
 
 /* ---- SGD step over one flat buffer (f32 / f64), in place
  * SGD::apply_simple_update / apply_momentum_update (engine/src/optim/sgd.rs:169-296):

@@ -55,10 +55,16 @@ SIGNATURES = {
                                       _vp]),
     "mtb200_token_log_probs_bwd": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _f64, _vp, _vp, _vp, _vp,
                                           _i64, _vp, _vp, _vp]),
+    "mtb200_token_log_probs_bwd_ex": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _f64, _vp, _vp, _vp, _vp,
+                                             _i64, _vp, _vp, _vp, _i64]),
     "mtb200_distill": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp, _vp,
                               _vp, _vp]),
     "mtb200_distill_bwd": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp,
                                   _vp]),
+    "mtb200_distill_ex": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp, _vp,
+                                 _vp, _vp, _i64]),
+    "mtb200_distill_bwd_ex": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i32, _f64, _i32, _f32, _vp, _vp,
+                                     _vp, _i64]),
     "mtb200_batch_norm_fwd": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _f64, _f64, _vp, _vp, _vp]),
     "mtb200_batch_norm_bwd": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "mtb200_dropout_mask": (_i32, [_vp, _i32, _i64, _f64, C.c_uint64, C.c_uint64, _vp]),

@@ -407,8 +407,12 @@ class Backend:
 
     @staticmethod
     def _grad_like(logits: torch.Tensor, rows: int, vocab: int, ld: int) -> torch.Tensor:
-        """A gradient buffer with the logits' row stride and offset within 16 bytes, so that both move in whole vectors."""
+        """A gradient buffer whose rows start at the logits' offsets within 16 bytes, so that both move in whole vectors.  It
+        has the logits' row stride where the vocabulary is padded; where a row lies further from the next than its own
+        length (a slice, such as the last position of every sequence), the shortest stride with these offsets."""
         off = (logits.data_ptr() & 15) // logits.element_size()
+        if ld >= 2 * vocab:
+            ld = vocab + (ld - vocab) % (16 // logits.element_size())
         if (off == 0 and ld == vocab) or rows == 0:
             return torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
         flat = torch.empty(off + (rows - 1) * ld + vocab, dtype=logits.dtype, device=logits.device)
@@ -456,7 +460,7 @@ class Backend:
                             d_top: Optional[torch.Tensor] = None, temperature: float = 1.0,
                             ignore_index: Optional[int] = None) -> torch.Tensor:
         """Gradient with respect to ``logits`` of :meth:`token_log_probs`, given the gradients of its outputs (any may be
-        ``None``) and what it returned; laid out in memory as the logits are, in their type."""
+        ``None``) and what it returned, in the logits' type.  Its rows are dense, with the logits' padding between them."""
         what = "token_log_probs_bwd"
         code, rows, vocab, ld = self._logit_rows(what, logits)
         self._vector(what, tokens, (rows,), (torch.int32, torch.int64))
@@ -474,11 +478,11 @@ class Backend:
             self._vector(what, d_top, (rows, top), f32)
         grad = self._grad_like(logits, rows, vocab, ld)
         self._bind_stream()
-        check(self.lib.mtb200_token_log_probs_bwd(
+        check(self.lib.mtb200_token_log_probs_bwd_ex(
             self._h, code, rows, vocab, logits.data_ptr(), ld, _ptr(tokens), I32 if tokens is None else _DTYPES[tokens.dtype],
             ignore_index is not None, ignore_index or 0, temperature, _ptr(stats), _ptr(d_log_probs),
             _ptr(entropy) if d_entropy is not None else None, _ptr(d_entropy), top, _ptr(top_indices) if top else None,
-            _ptr(d_top) if top else None, grad.data_ptr()))
+            _ptr(d_top) if top else None, grad.data_ptr(), grad.stride(0)))
         self.launches += 1
         return grad
 
@@ -510,11 +514,12 @@ class Backend:
         loss = row_loss if red == 2 else torch.empty(1, dtype=torch.float32, device=logits.device)
         grad = self._grad_like(logits, rows, vocab, ld) if want_grad else None
         self._bind_stream()
-        check(self.lib.mtb200_distill(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
-                                      _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
-                                      _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream, _ptr(upstream_rows),
-                                      _ptr(row_loss), None if red == 2 else _ptr(loss), _ptr(stats),
-                                      grad.data_ptr() if want_grad and grad.numel() else None))
+        check(self.lib.mtb200_distill_ex(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
+                                         _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
+                                         _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream, _ptr(upstream_rows),
+                                         _ptr(row_loss), None if red == 2 else _ptr(loss), _ptr(stats),
+                                         grad.data_ptr() if want_grad and grad.numel() else None,
+                                         grad.stride(0) if want_grad else vocab))
         self.launches += 1 if red == 2 else 2
         return loss, grad
 
@@ -526,10 +531,10 @@ class Backend:
                                                                reduction, upstream_rows, stats)
         grad = self._grad_like(logits, rows, vocab, ld)
         self._bind_stream()
-        check(self.lib.mtb200_distill_bwd(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
-                                          _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
-                                          _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream, _ptr(upstream_rows),
-                                          _ptr(stats), grad.data_ptr()))
+        check(self.lib.mtb200_distill_bwd_ex(self._h, code, rows, vocab, logits.data_ptr(), ld, top, _ptr(teacher_indices),
+                                             _DTYPES[teacher_indices.dtype], _ptr(teacher_logits),
+                                             _LOGIT_DTYPES[teacher_logits.dtype], temperature, red, upstream,
+                                             _ptr(upstream_rows), _ptr(stats), grad.data_ptr(), grad.stride(0)))
         self.launches += 1
         return grad
 

@@ -60,7 +60,7 @@ struct Block {
 // The same for kernels whose blocks do not meet: `whole` rows with a block each, then the others in `parts` parts.
 template <int G>
 struct Cut {
-  long long row;  // -1: nothing to do
+  int row;  // -1: nothing to do
   int part, parts;
   __device__ __forceinline__ Cut(int rows, int whole, int cut_parts) {
     const unsigned unit = G == 32 ? blockIdx.x * Block<G>::ROWS + Block<G>::slot() : blockIdx.x;
@@ -70,7 +70,7 @@ struct Cut {
       parts = 1;
     } else {
       const unsigned more = unit - whole;
-      row = static_cast<long long>(whole) + more / static_cast<unsigned>(cut_parts);
+      row = whole + static_cast<int>(more / static_cast<unsigned>(cut_parts));
       part = more % static_cast<unsigned>(cut_parts);
       parts = cut_parts;
       if (row >= rows) row = -1;
@@ -193,7 +193,7 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, (TOP ? 1024 : 1536) 
 struct ScoreGradArgs {
   const void* logits;
   void* dlogits;
-  long long ld;
+  long long ld, ld_grad;
   int rows, vocab, top, parts, whole, same_phase;
   IndexArray tokens;
   int has_ignore;
@@ -204,9 +204,16 @@ struct ScoreGradArgs {
   uint32_t* bad_label;
 };
 
+// Blocks of a gradient kernel on an SM, which limit its registers: warps on 20000 x 1000 f32 with the entropy's gradient take 55 us
+// in four blocks and 63 in the three that fit without a limit, 20000 x 2000 bf16 without it 55 and 64.
+template <typename T, int G, bool ENT>
+constexpr int grad_blocks() {
+  return G == 512 ? 4 : sizeof(T) == 2 && ENT ? 1 : G == 32 ? 4 : sizeof(T) == 4 && !ENT ? 9 : 8;
+}
+
 // dx = (1/T) [ sum of weights at given indices - p (sum of all weights) - g_H p (log p + H) ], one read, one write.
 template <typename T, int G, bool ENT>
-static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) token_scores_grad_kernel(ScoreGradArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, grad_blocks<T, G, ENT>()) token_scores_grad_kernel(ScoreGradArgs a) {
   __shared__ __align__(16) int all_idx[Block<G>::ROWS][VOCAB_TOP_MAX + 4];
   __shared__ float all_weight[Block<G>::ROWS][VOCAB_TOP_MAX + 1];
   __shared__ float fold[Group<G>::WARPS];
@@ -214,11 +221,11 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) to
   float* weight = all_weight[Block<G>::slot()];
   const Cut<G> cut(a.rows, a.whole, a.parts);
   const int part = cut.part;
-  const long long r = cut.row;
+  const int r = cut.row;
   const int tid = Group<G>::rank();
   if (r < 0) return;
-  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
+  const T* row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
+  T* dx = static_cast<T*>(a.dlogits) + static_cast<long long>(r) * a.ld_grad;
   const RowPart<T> p = row_part(row, a.vocab, part, cut.parts);
   const long long token = a.tokens.p ? a.tokens.at(r) : -1;
   if (a.tokens.p && a.has_ignore && token == a.ignore) {
@@ -236,12 +243,12 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) to
       j = good && a.d_log_probs ? static_cast<int>(token) : -1;
       w = j >= 0 ? a.d_log_probs[r] : 0.0f;
     } else {
-      j = a.top_indices[r * a.top + e - 1];
+      j = a.top_indices[static_cast<long long>(r) * a.top + e - 1];
       if (j < 0 || j >= a.vocab) {  // -1: no entry
         if (j >= a.vocab) atomicOr(a.bad_label, 1u);
         j = -1;
       }
-      w = j >= 0 ? a.d_top[r * a.top + e - 1] : 0.0f;
+      w = j >= 0 ? a.d_top[static_cast<long long>(r) * a.top + e - 1] : 0.0f;
     }
     idx[e] = j;
     weight[e] = w * a.inv_t;
@@ -265,7 +272,7 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) to
 struct DistillArgs {
   const void* logits;
   void* dlogits;           // forward: nullptr = loss only
-  long long ld;
+  long long ld, ld_grad;
   int rows, vocab, top, parts, whole, same_phase;
   IndexArray index;
   RealArray value;
@@ -319,10 +326,19 @@ __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, 
   return true;
 }
 
+// The row's gradient, for the second look at the row: the compiler is kept from computing the address before the first look,
+// where its two registers are not to be had (1021 x 50257 f32 with 100 entries 102 us instead of 107, 300 x 50257 bf16 with 700
+// entries 77 instead of 86).
+template <typename T>
+__device__ __forceinline__ T* grad_row_late(const DistillArgs& a, int r) {
+  asm volatile("" : "+r"(r));
+  return static_cast<T*>(a.dlogits) + static_cast<long long>(r) * a.ld_grad;
+}
+
 // Loss per row, T^2 sum_k q_k (log q_k - log p_idx_k), and with GRAD the gradient: the row's statistics, then a second
-// look at the row while it is in L2.
+// look at the row while it is in L2.  Warps keep to five blocks on an SM (20000 x 1000 f32: 48 us, 53 in four).
 template <typename T, int G, bool GRAD>
-static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(DistillArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, G == 32 && GRAD ? 5 : 0) distill_kernel(DistillArgs a) {
   using L = LogitType<T>;
   __shared__ RowStat sm[Group<G>::WARPS + 1], parts_st[MAX_PARTS];
   __shared__ __align__(16) int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
@@ -332,11 +348,10 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
   float *q = all_q[Block<G>::slot()], *dv = all_dv[Block<G>::slot()];
   cg::cluster_group cluster = cg::this_cluster();
   const int part = Block<G>::part(a.parts);
-  const long long r = Block<G>::row(a.rows, a.parts);
+  const int r = static_cast<int>(Block<G>::row(a.rows, a.parts));
   const int tid = Group<G>::rank();
   if (r < 0) return;
-  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dx = GRAD ? static_cast<T*>(a.dlogits) + r * a.ld : nullptr;
+  const T* row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
 
   float ln_sq;
@@ -348,7 +363,7 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
         a.stats[2 * r + 1] = 0.0f;
       }
     }
-    if (GRAD) zero_grad<T, G>(p, dx, a.same_phase);
+    if (GRAD) zero_grad<T, G>(p, grad_row_late<T>(a, r), a.same_phase);
     return;
   }
   const bool split = G > 32 && a.parts > 1;
@@ -387,6 +402,7 @@ static __global__ void __launch_bounds__(Block<G>::THREADS) distill_kernel(Disti
     const float scale = a.upstream_rows ? a.scale * a.upstream_rows[r] : a.scale;
     g.a = isnan(ln_sq) ? NAN : scale;
     g.b = 0.0f;
+    T* dx = grad_row_late<T>(a, r);
     dense_grad<T, G, false>(p, dx, a.c, g, a.same_phase);
     for (int e = tid; e < a.top; e += G) q[e] *= -scale;
     Group<G>::sync();
@@ -414,9 +430,8 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = tid - 32;
   const bool entry = e >= 0 && e < a.top, entry_warp = warp > 0 && 32 * (warp - 1) < a.top;
   const int part = Block<G>::part(a.parts);
-  const long long r = Block<G>::row(a.rows, a.parts);
-  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
+  const int r = static_cast<int>(Block<G>::row(a.rows, a.parts));
+  const T* row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
   const RowPart<T> p = row_part(row, a.vocab, part, a.parts);
   if (tid == 0) {
     mbar_init(smem_u32(&arrived), 1);
@@ -427,10 +442,10 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
   int mine = -1;
   float v = -INFINITY;
   if (entry) {
-    const long long j = a.index.at(r * a.top + e);
+    const long long j = a.index.at(static_cast<long long>(r) * a.top + e);
     if (j >= 0 && j < a.vocab) mine = static_cast<int>(j);
     else if (j != -1 && part == 0) atomicOr(a.bad_label, 1u);
-    if (mine >= 0) v = a.value.at(r * a.top + e);
+    if (mine >= 0) v = a.value.at(static_cast<long long>(r) * a.top + e);
     idx[e] = mine;
     twice[e] = 0;
   }
@@ -443,7 +458,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
         a.stats[2 * r + 1] = 0.0f;
       }
     }
-    zero_grad<T, G>(p, dx, a.same_phase);
+    zero_grad<T, G>(p, static_cast<T*>(a.dlogits) + static_cast<long long>(r) * a.ld_grad, a.same_phase);
     return;
   }
   if (a.parts > 1) cluster.barrier_arrive();  // waited for before another block is sent to
@@ -501,6 +516,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
   bool teacher_nan = false;  // a NaN or +inf among the teacher's values is in the sum of its warp
   for (int k = 1; k < WARPS && 32 * (k - 1) < a.top; ++k) teacher_nan = teacher_nan || isnan(teacher_sm[k].s);
   g.a = teacher_nan ? NAN : scale;
+  T* dx = grad_row_late<T>(a, r);
   dense_grad<T, G, false>(p, dx, a.c, g, a.same_phase);
   if (entry_warp && part == 0) {
     // log q - log p with the two maxima taken out first: nearly equal distributions lose nothing to the logarithms' size
@@ -534,7 +550,7 @@ static __global__ void __launch_bounds__(512, 3) distill_cluster_kernel(DistillA
 }
 
 template <typename T, int G>
-static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) distill_grad_kernel(DistillArgs a) {
+static __global__ void __launch_bounds__(Block<G>::THREADS, grad_blocks<T, G, false>()) distill_grad_kernel(DistillArgs a) {
   __shared__ __align__(16) int all_idx[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float all_q[Block<G>::ROWS][TEACHER_ROOM<G>];
   __shared__ float fold[Group<G>::WARPS];
@@ -542,10 +558,10 @@ static __global__ void __launch_bounds__(Block<G>::THREADS, G == 512 ? 4 : 1) di
   float* q = all_q[Block<G>::slot()];
   const Cut<G> cut(a.rows, a.whole, a.parts);
   const int part = cut.part;
-  const long long r = cut.row;
+  const int r = cut.row;
   if (r < 0) return;
-  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dx = static_cast<T*>(a.dlogits) + r * a.ld;
+  const T* row = static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld;
+  T* dx = static_cast<T*>(a.dlogits) + static_cast<long long>(r) * a.ld_grad;
   const RowPart<T> p = row_part(row, a.vocab, part, cut.parts);
   float ln_sq;
   if (!load_teacher<G>(a, r, part == 0, idx, q, nullptr, fold, &ln_sq)) {
@@ -598,8 +614,10 @@ static int32_t check_rows(const char* what, int32_t dtype, int64_t rows, int64_t
     return fail(MTB200_ERR_INVALID, "%s: temperature must be positive and finite, got %g", what, temperature);
   return MTB200_OK;
 }
-static int32_t check_grad(const char* what, int32_t dtype, const void* logits, const void* dlogits) {
+static int32_t check_grad(const char* what, int32_t dtype, int64_t vocab, const void* logits, const void* dlogits, int64_t ld_grad) {
   if (dlogits == logits) return fail(MTB200_ERR_INVALID, "%s does not work in place", what);
+  if (ld_grad < vocab)
+    return fail(MTB200_ERR_INVALID, "%s: row stride %lld of the gradient is less than the vocabulary", what, (long long)ld_grad);
   if (reinterpret_cast<uintptr_t>(dlogits) % logit_size(dtype)) return fail(MTB200_ERR_INVALID, "%s: misaligned gradient", what);
   return MTB200_OK;
 }
@@ -735,8 +753,9 @@ static int32_t by_type_and_group(int32_t dtype, int group, F f) {
   if (dtype == MTB200_F16) return with(__half());
   return with(__nv_bfloat16());
 }
-static int same_phase(const void* x, const void* y) {
-  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+// whether each row starts at the same offset within 16 bytes in both matrices
+static int same_phase(const void* x, int64_t ldx, const void* y, int64_t ldy, int32_t dtype) {
+  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0 && (ldx - ldy) * int64_t(logit_size(dtype)) % 16 == 0;
 }
 
 }  // namespace mtb
@@ -778,11 +797,11 @@ int32_t mtb200_token_log_probs(mtb200_handle h, int32_t dtype, int64_t rows, int
   return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_scores<decltype(element), group_of(tag)>(h, a); });
 }
 
-int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
-                                   const void* tokens, int32_t token_dtype, int32_t has_ignore, int64_t ignore_index,
-                                   double temperature, const float* stats, const float* d_log_probs, const float* entropy,
-                                   const float* d_entropy, int64_t top, const int32_t* top_indices, const float* d_top,
-                                   void* dlogits) {
+int32_t mtb200_token_log_probs_bwd_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                                      const void* tokens, int32_t token_dtype, int32_t has_ignore, int64_t ignore_index,
+                                      double temperature, const float* stats, const float* d_log_probs, const float* entropy,
+                                      const float* d_entropy, int64_t top, const int32_t* top_indices, const float* d_top,
+                                      void* dlogits, int64_t ld_grad) {
   MTB_CHECK_HANDLE(h);
   const char* what = "token_log_probs_bwd";
   if (int32_t rc = check_rows(what, dtype, rows, vocab, logits, ld, temperature)) return rc;
@@ -793,24 +812,32 @@ int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows,
   if (rows == 0 || vocab == 0) return MTB200_OK;
   if (!logits || !stats || !dlogits || (d_log_probs && !tokens) || (d_entropy && !entropy) || (top && (!top_indices || !d_top)))
     return fail(MTB200_ERR_INVALID, "%s: null pointer", what);
-  if (int32_t rc = check_grad(what, dtype, logits, dlogits)) return rc;
+  if (int32_t rc = check_grad(what, dtype, vocab, logits, dlogits, ld_grad)) return rc;
   ScoreGradArgs a = {};
-  a.logits = logits; a.dlogits = dlogits; a.ld = ld; a.rows = int(rows); a.vocab = int(vocab); a.top = int(top);
+  a.logits = logits; a.dlogits = dlogits; a.ld = ld; a.ld_grad = ld_grad; a.rows = int(rows); a.vocab = int(vocab); a.top = int(top);
   a.tokens = {tokens, token_dtype == MTB200_I64};
   a.has_ignore = has_ignore != 0; a.ignore = ignore_index;
   a.inv_t = float(1.0 / temperature); a.c = float(1.4426950408889634 / temperature);
   a.stats = stats; a.entropy = entropy; a.d_log_probs = d_log_probs; a.d_entropy = d_entropy; a.d_top = d_top;
   a.top_indices = top_indices; a.bad_label = h->status + 1;
-  a.same_phase = same_phase(logits, dlogits);
+  a.same_phase = same_phase(logits, ld, dlogits, ld_grad, dtype);
   const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), true, MID_BYTES);
   a.parts = plan.parts;
   return by_type_and_group(dtype, plan.group, [&](auto element, auto tag) { return launch_score_grad<decltype(element), group_of(tag)>(h, a); });
+}
+int32_t mtb200_token_log_probs_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                                   const void* tokens, int32_t token_dtype, int32_t has_ignore, int64_t ignore_index,
+                                   double temperature, const float* stats, const float* d_log_probs, const float* entropy,
+                                   const float* d_entropy, int64_t top, const int32_t* top_indices, const float* d_top,
+                                   void* dlogits) {
+  return mtb200_token_log_probs_bwd_ex(h, dtype, rows, vocab, logits, ld, tokens, token_dtype, has_ignore, ignore_index, temperature,
+                                       stats, d_log_probs, entropy, d_entropy, top, top_indices, d_top, dlogits, ld);
 }
 
 static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, int64_t rows, int64_t vocab, const void* logits,
                             int64_t ld, int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
                             int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
-                            const float* upstream_rows, void* dlogits, DistillArgs* a, int* group) {
+                            const float* upstream_rows, void* dlogits, int64_t ld_grad, DistillArgs* a, int* group) {
   if (int32_t rc = check_rows(what, dtype, rows, vocab, logits, ld, temperature)) return rc;
   if (int32_t rc = check_index(what, index_dtype)) return rc;
   if (!logit_size(teacher_dtype))
@@ -822,30 +849,30 @@ static int32_t distill_args(mtb200_handle h, const char* what, int32_t dtype, in
   if (rows > 0 && vocab > 0 && (!logits || (top && (!teacher_indices || !teacher_logits))))
     return fail(MTB200_ERR_INVALID, "%s: null pointer", what);
   if (dlogits)
-    if (int32_t rc = check_grad(what, dtype, logits, dlogits)) return rc;
+    if (int32_t rc = check_grad(what, dtype, vocab, logits, dlogits, ld_grad)) return rc;
   *a = {};
-  a->logits = logits; a->dlogits = dlogits; a->ld = ld; a->rows = int(rows); a->vocab = int(vocab); a->top = int(top);
+  a->logits = logits; a->dlogits = dlogits; a->ld = ld; a->ld_grad = ld_grad; a->rows = int(rows); a->vocab = int(vocab); a->top = int(top);
   a->index = {teacher_indices, index_dtype == MTB200_I64};
   a->value = {teacher_logits, teacher_dtype};
   a->t = float(temperature); a->c = float(1.4426950408889634 / temperature);
   a->scale = float(temperature * (reduction == MTB200_REDUCE_MEAN && rows ? 1.0 / double(rows) : 1.0) * double(upstream));
   a->upstream_rows = upstream_rows; a->status = h->status; a->bad_label = h->status + 1;
-  a->same_phase = same_phase(logits, dlogits);
+  a->same_phase = same_phase(logits, ld, dlogits, ld_grad, dtype);
   const RowPlan plan = plan_rows(h, rows, vocab * int64_t(logit_size(dtype)), top <= TEACHER_WARP_MAX, MID_BYTES);
   a->parts = plan.parts;
   *group = plan.group;
   return MTB200_OK;
 }
 
-int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, int64_t top,
-                       const void* teacher_indices, int32_t index_dtype, const void* teacher_logits, int32_t teacher_dtype,
-                       double temperature, int32_t reduction, float upstream, const float* upstream_rows, float* row_loss,
-                       float* loss, float* stats, void* dlogits) {
+int32_t mtb200_distill_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, int64_t top,
+                          const void* teacher_indices, int32_t index_dtype, const void* teacher_logits, int32_t teacher_dtype,
+                          double temperature, int32_t reduction, float upstream, const float* upstream_rows, float* row_loss,
+                          float* loss, float* stats, void* dlogits, int64_t ld_grad) {
   MTB_CHECK_HANDLE(h);
   DistillArgs a;
   int group;
   if (int32_t rc = distill_args(h, "distill", dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype, teacher_logits,
-                                teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a, &group))
+                                teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, ld_grad, &a, &group))
     return rc;
   if ((rows > 0 && !row_loss) || (reduction != MTB200_REDUCE_NONE && !loss)) return fail(MTB200_ERR_INVALID, "null loss pointer");
   a.row_loss = row_loss;
@@ -868,22 +895,36 @@ int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t voc
   }
   return MTB200_OK;
 }
+int32_t mtb200_distill(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, int64_t top,
+                       const void* teacher_indices, int32_t index_dtype, const void* teacher_logits, int32_t teacher_dtype,
+                       double temperature, int32_t reduction, float upstream, const float* upstream_rows, float* row_loss,
+                       float* loss, float* stats, void* dlogits) {
+  return mtb200_distill_ex(h, dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype, teacher_logits, teacher_dtype,
+                           temperature, reduction, upstream, upstream_rows, row_loss, loss, stats, dlogits, ld);
+}
 
-int32_t mtb200_distill_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
-                           int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
-                           int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
-                           const float* upstream_rows, const float* stats, void* dlogits) {
+int32_t mtb200_distill_bwd_ex(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                              int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                              int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                              const float* upstream_rows, const float* stats, void* dlogits, int64_t ld_grad) {
   MTB_CHECK_HANDLE(h);
   DistillArgs a;
   int group;
   if (int32_t rc = distill_args(h, "distill_bwd", dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype,
-                                teacher_logits, teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, &a, &group))
+                                teacher_logits, teacher_dtype, temperature, reduction, upstream, upstream_rows, dlogits, ld_grad, &a, &group))
     return rc;
   if (rows == 0 || vocab == 0) return MTB200_OK;
   if (!stats || !dlogits) return fail(MTB200_ERR_INVALID, "distill_bwd: null pointer");
   a.stats = const_cast<float*>(stats);
   return by_type_and_group(dtype, group,
                            [&](auto element, auto tag) { return launch_distill<decltype(element), group_of(tag)>(h, a); });
+}
+int32_t mtb200_distill_bwd(mtb200_handle h, int32_t dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                           int64_t top, const void* teacher_indices, int32_t index_dtype, const void* teacher_logits,
+                           int32_t teacher_dtype, double temperature, int32_t reduction, float upstream,
+                           const float* upstream_rows, const float* stats, void* dlogits) {
+  return mtb200_distill_bwd_ex(h, dtype, rows, vocab, logits, ld, top, teacher_indices, index_dtype, teacher_logits, teacher_dtype,
+                               temperature, reduction, upstream, upstream_rows, stats, dlogits, ld);
 }
 
 }  // extern "C"

@@ -77,6 +77,21 @@ def test_gradient_buffers_follow_the_logits():
         assert g.shape == x.shape and g.stride() == x.stride() and (g.data_ptr() ^ x.data_ptr()) & 15 == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,seq,vocab", [(4, 300, 50), (7, 33, 1), (3, 3, 77), (5, 2, 24)])
+def test_gradient_buffers_of_slices_are_no_larger_than_their_rows(dtype, rows, seq, vocab):
+    """The last position of every sequence: the gradient holds these rows, not the whole of what they were taken from, and
+    every row starts at its logits' offset within 16 bytes."""
+    from minitensor_b200.backend import Backend
+    for off in (0, 1):
+        x = torch.zeros(rows * seq * vocab + off, dtype=dtype)[off:].view(rows, seq, vocab)[:, -1]
+        g = Backend._grad_like(x, rows, vocab, x.stride(0))
+        size, unit = g.element_size(), 16 // g.element_size()
+        assert g.shape == x.shape and g.dtype == dtype and g.stride(1) == 1 and g.stride(0) >= vocab
+        assert g.untyped_storage().nbytes() <= (rows * (vocab + unit) + unit) * size
+        assert all((g[r].data_ptr() - x[r].data_ptr()) % 16 == 0 for r in range(rows))
+
+
 def test_nn_refusals_come_before_the_device():
     import minitensor_b200.nn as nn
     from minitensor_b200.tensor import Tensor

@@ -677,3 +677,93 @@ def test_more_alternatives_from_call_to_call_in_a_new_process():
     script = _RISING_TOPS.format(root=ROOT, tests=os.path.join(ROOT, "tests"))
     run = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,seq,vocab", [(6, 5, 1003), (160, 3, 515), (3, 4, 50257), (400, 2, 9001)])
+def test_gradients_of_the_last_positions(be, dtype, rows, seq, vocab):
+    """Logits whose rows lie further apart than they are long; their gradient takes the room of its own rows."""
+    x = logits_for(rows * seq, vocab, 0, dtype, 31).view(rows, seq, vocab)[:, -1]
+    tokens = torch.arange(rows, device="cuda") % vocab
+    check_scores(be, x, tokens, 1.0, 5)
+    check_score_grad(be, x, tokens, 0.9, 5)
+    idx, val = teacher_for(rows, vocab, 11, 6)
+    check_distill(be, x, idx, val, 1.5)
+    _, grad = be.distillation_loss(x, idx, val)
+    assert grad.untyped_storage().nbytes() <= (rows * (vocab + 8) + 8) * grad.element_size()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [5, 1001, 20011])
+def test_c_entries_with_two_row_strides(be, dtype, vocab):
+    """Logits and gradient with row strides that differ by whole vectors or by single elements, either one the longer:
+    only the vocabulary's columns of the gradient are written, with the values that a dense gradient gets."""
+    from minitensor_b200 import _lib
+    from minitensor_b200.backend import _LOGIT_DTYPES
+    rows, top = 7, 4
+    code, unit = _LOGIT_DTYPES[dtype], 16 // torch.empty(0, dtype=dtype).element_size()
+    idx, val = teacher_for(rows, vocab, top, 4)
+    tokens = torch.arange(rows, device="cuda") % vocab
+    d = torch.randn(rows, device="cuda")
+    for ld, ldg in [(vocab, vocab), (vocab + 3, vocab), (vocab, vocab + 5), (vocab + 4 * unit, vocab), (vocab, vocab + 2 * unit)]:
+        x = torch.randn(rows * ld, device="cuda").to(dtype).view(rows, ld)[:, :vocab]
+        fwd = be.token_log_probs(x, tokens, entropy=True)
+        want_s = be.token_log_probs_bwd(x, tokens, fwd.stats, d_log_probs=d, entropy=fwd.entropy, d_entropy=d)
+        row_loss, loss, stats = torch.empty(rows, device="cuda"), torch.empty(1, device="cuda"), torch.empty(rows, 2, device="cuda")
+        _, want_d = be.distillation_loss(x, idx, val, stats=stats)
+        want_b = be.distillation_loss_bwd(x, idx, val, stats)
+        out = torch.empty(rows * ldg + 16, dtype=dtype, device="cuda")
+        be._bind_stream()
+
+        def kept(want):
+            be.sync()
+            rest = out[:rows * ldg].view(rows, ldg)
+            assert torch.equal(rest[:, :vocab], want)
+            assert (rest[:, vocab:] == 77.0).all() and (out[rows * ldg:] == 77.0).all()
+            out.fill_(77.0)
+        out.fill_(77.0)
+        _lib.check(be.lib.mtb200_token_log_probs_bwd_ex(
+            be._h, code, rows, vocab, x.data_ptr(), ld, tokens.data_ptr(), _lib.I64, 0, 0, 1.0, fwd.stats.data_ptr(), d.data_ptr(),
+            fwd.entropy.data_ptr(), d.data_ptr(), 0, None, None, out.data_ptr(), ldg))
+        kept(want_s)
+        args = [be._h, code, rows, vocab, x.data_ptr(), ld, top, idx.data_ptr(), _lib.I32, val.data_ptr(), _lib.F32, 1.0, 1, 1.0, None]
+        _lib.check(be.lib.mtb200_distill_ex(*args, row_loss.data_ptr(), loss.data_ptr(), stats.data_ptr(), out.data_ptr(), ldg))
+        kept(want_d)
+        _lib.check(be.lib.mtb200_distill_bwd_ex(*args, stats.data_ptr(), out.data_ptr(), ldg))
+        kept(want_b)
+        for call in (lambda: be.lib.mtb200_distill_bwd_ex(*args, stats.data_ptr(), out.data_ptr(), vocab - 1),
+                     lambda: be.lib.mtb200_distill_ex(*args, row_loss.data_ptr(), loss.data_ptr(), None, out.data_ptr(), vocab - 1),
+                     lambda: be.lib.mtb200_token_log_probs_bwd_ex(
+                         be._h, code, rows, vocab, x.data_ptr(), ld, None, _lib.I32, 0, 0, 1.0, stats.data_ptr(), None, None, None, 0,
+                         None, None, out.data_ptr(), vocab - 1)):
+            assert call() == _lib.ERR_INVALID and "row stride" in _lib.last_error()
+
+
+def test_gradients_beyond_32_bits(be):
+    """Gradients whose rows lie behind element 2^31, by the C entries with one row stride for both matrices."""
+    from minitensor_b200 import _lib
+    rows, vocab, ld, top = 5, 20001, 2 ** 29 + 8, 9
+    size = (rows - 1) * ld + vocab
+    x, out = (torch.zeros(size, dtype=torch.bfloat16, device="cuda").as_strided((rows, vocab), (ld, 1)) for _ in range(2))
+    x.copy_(logits_for(rows, vocab, 0, torch.bfloat16, 6))
+    idx, val = teacher_for(rows, vocab, top, 6)
+    tokens = torch.arange(rows, device="cuda")
+    d = torch.randn(rows, device="cuda")
+    fwd = be.token_log_probs(x, tokens)
+    want_s = be.token_log_probs_bwd(x, tokens, fwd.stats, d_log_probs=d)
+    row_loss, loss, stats = torch.empty(rows, device="cuda"), torch.empty(1, device="cuda"), torch.empty(rows, 2, device="cuda")
+    _, want_d = be.distillation_loss(x, idx, val, stats=stats)
+    want_b = be.distillation_loss_bwd(x, idx, val, stats)
+    be._bind_stream()
+    _lib.check(be.lib.mtb200_token_log_probs_bwd(
+        be._h, _lib.BF16, rows, vocab, x.data_ptr(), ld, tokens.data_ptr(), _lib.I64, 0, 0, 1.0, fwd.stats.data_ptr(), d.data_ptr(), None,
+        None, 0, None, None, out.data_ptr()))
+    be.sync()
+    assert torch.equal(out, want_s)
+    args = [be._h, _lib.BF16, rows, vocab, x.data_ptr(), ld, top, idx.data_ptr(), _lib.I32, val.data_ptr(), _lib.F32, 1.0, 1, 1.0, None]
+    for want, call in ((want_d, lambda: be.lib.mtb200_distill(*args, row_loss.data_ptr(), loss.data_ptr(), stats.data_ptr(), out.data_ptr())),
+                       (want_b, lambda: be.lib.mtb200_distill_bwd(*args, stats.data_ptr(), out.data_ptr()))):
+        out.zero_()
+        _lib.check(call())
+        be.sync()
+        assert torch.equal(out, want)
