@@ -100,7 +100,9 @@ int32_t mtb200_set_stream(mtb200_handle h, void* cuda_stream);
  * with them the whole GEMM; leaving it a few SMs costs less than that. */
 int32_t mtb200_set_gemm_sm_limit(mtb200_handle h, int32_t sms);
 /* CudaBackend::synchronize (engine/src/backends/cuda/mod.rs:153-161); also
- * reports MTB200_ERR_DEVICE_WAIT if a kernel recorded an expired wait. */
+ * reports MTB200_ERR_DEVICE_WAIT if a kernel recorded an expired wait; the message's
+ * role tells which: 1..3 products and conv2d's weight gradient, 4..11 conv2d,
+ * 15 mtb200_selftest_wait_expiry, 16 the distillation step. */
 int32_t mtb200_sync(mtb200_handle h);
 /* Per-launch timing, the device-side analogue of the reference's manual
  * OperationProfiler (engine/src/debug.rs:273-352).  While enabled, every kernel

@@ -307,7 +307,7 @@ int32_t mtb200_sync(mtb200_handle h) {
     MTB_CUDA(cudaStreamSynchronize(h->stream));
     if (wait_code)
       return fail(MTB200_ERR_DEVICE_WAIT,
-                  "a bounded wait inside a GEMM kernel ran out (role %u, site %u); results are invalid",
+                  "a bounded wait inside a kernel ran out (role %u, site %u); results are invalid",
                   wait_code >> 8, wait_code & 0xffu);
     return fail(MTB200_ERR_BAD_LABEL, "a loss saw a class index or token outside [0, C)");
   }
@@ -754,7 +754,7 @@ int32_t mtb200_adam_step_counted(mtb200_handle h, int64_t n, float* param, const
 // ------------------------------------------------------------------ bounded-wait self-test
 namespace mtb {
 // One thread waits on a barrier that nothing signals, with the same loop shape as mbar_wait but a caller-chosen
-// limit, and reports the expiry through the status word exactly as the GEMM kernels' roles do (role 15, site 1).
+// limit, and reports the expiry through the status word exactly as the kernels' roles do (role 15, site 1).
 __global__ void wait_expiry_selftest_kernel(uint32_t* __restrict__ status, unsigned long long limit_ns) {
   __shared__ __align__(8) unsigned long long bar;
   const uint32_t b = smem_u32(&bar);

@@ -767,3 +767,15 @@ def test_gradients_beyond_32_bits(be):
         _lib.check(call())
         be.sync()
         assert torch.equal(out, want)
+
+
+def test_an_expired_wait_is_not_laid_on_the_products(be):
+    """The distillation step waits for messages between blocks and reports as the tensor kernels do; the message names
+    the role, and no kernel that it cannot know."""
+    from minitensor_b200._lib import Mtb200Error, check
+    be.sync()
+    check(be.lib.mtb200_selftest_wait_expiry(be._h, 1000))
+    with pytest.raises(Mtb200Error, match="role 15, site 1") as err:
+        be.sync()
+    assert "GEMM" not in str(err.value)
+    be.sync()
