@@ -71,7 +71,6 @@ struct LogitType;
 template <>
 struct LogitType<float> {
   static constexpr int VEC = 4;
-  static constexpr int KEY_SHIFT = 0;               // bits of an f32 sort key that are the same for every value
   static constexpr uint32_t NEG_INF_WORD = 0xff800000u;
   static __device__ __forceinline__ float up(float x) { return x; }
   static __device__ __forceinline__ float down(float x) { return x; }
@@ -102,7 +101,6 @@ struct LogitType<float> {
 template <>
 struct LogitType<__nv_bfloat16> {
   static constexpr int VEC = 8;
-  static constexpr int KEY_SHIFT = 16;
   static constexpr uint32_t NEG_INF_WORD = 0xff80ff80u;
   static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
@@ -143,7 +141,6 @@ struct LogitType<__nv_bfloat16> {
 template <>
 struct LogitType<__half> {
   static constexpr int VEC = 8;
-  static constexpr int KEY_SHIFT = 13;
   static constexpr uint32_t NEG_INF_WORD = 0xfc00fc00u;
   static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
