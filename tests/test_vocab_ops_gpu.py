@@ -779,3 +779,171 @@ def test_an_expired_wait_is_not_laid_on_the_products(be):
         be.sync()
     assert "GEMM" not in str(err.value)
     be.sync()
+
+
+# ------------------------------------------------------------------ special rows of long vocabularies
+def distill_bounds(x, idx, val, temperature):
+    """(row losses, gradient of their sum, tolerance of the losses, tolerance of the gradient but for its final rounding) in
+    64 bits.
+
+    With q = 2^(c dv) / S_q: the exponent carries the roundings of dv, c and their product, 3 U |dv / T| where |dv / T| is at
+    most |ln q| + ln(entries); the power of two 4 U and the division 2 U.  S_q has the mean of that over q, at most
+    3 U * 2 ln(entries + 1) + 4 U, and no more than 44 additions on the way of any term (8 a thread, 5 + 5 by shuffles, 16
+    warps, a few to spare).  A term of the loss is q times a bracket of ln q - ln p, in whose pieces no number is larger than
+    |ln q| + |ln p| + 2 ln(entries) + 2 ln(vocabulary): 8 roundings of that, the errors of q, ln S_q and ln S, and 44
+    additions.  Weights with the same index are added one after the other: one U of their sum for each."""
+    rows, vocab = x.shape
+    top = idx.shape[1]
+    U = ref.U
+    loss, grad = ref.distill64(x, idx, val, temperature)
+    _, lp = ref.softmax64(x, temperature)
+    q = ref.teacher64(idx, val, temperature)
+    at = idx.long().clamp(min=0)
+    lpk = lp.gather(1, at)
+    lpk = torch.where((q > 0) & torch.isfinite(lpk), lpk.abs(), torch.zeros_like(q))
+    lqk = torch.where(q > 0, q, torch.ones_like(q)).log().abs()
+    e_q = U * (6 * math.log(top + 1) + 48)
+    rel_q = U * (3 * (lqk + math.log(top + 1)) + 8) + e_q
+    size = lqk + lpk + 2 * math.log(top + 1) + 2 * math.log(vocab + 1)
+    tol = temperature ** 2 * (q * (size * (52 * U + rel_q) + e_q + ref.sum_error(vocab))).sum(1)
+    count = torch.zeros_like(grad).scatter_add_(1, at, (idx >= 0).double())
+    mass = torch.zeros_like(grad).scatter_add_(1, at, q)
+    more = torch.zeros_like(grad).scatter_add_(1, at, q * (rel_q + 2 * U)) + count * U * mass
+    return loss, grad, tol, more * temperature
+
+
+def check_special_distill(be, x, idx, val, temperature, nan_rows=()):
+    rows, vocab = x.shape
+    good = torch.tensor([r not in nan_rows for r in range(rows)], device="cuda")
+    want, grad64, tol, more = distill_bounds(x[good], idx[good], val[good], temperature)
+    p, lp = ref.softmax64(x[good], temperature)
+    weights = 0.5 + torch.rand(rows, device="cuda")
+    for reduction in ("none", "mean", "sum"):
+        if nan_rows and reduction != "none":
+            continue
+        kw = dict(temperature=temperature, reduction=reduction)
+        stats = torch.empty(rows, 2, device="cuda")
+        loss, grad = be.distillation_loss(x, idx, val, upstream=0.5, upstream_rows=weights, stats=stats, **kw)
+        only, _ = be.distillation_loss(x, idx, val, want_grad=False, **kw)
+        again = be.distillation_loss_bwd(x, idx, val, stats, upstream=0.5, upstream_rows=weights, **kw)
+        be.sync()
+        f = 1.0 / rows if reduction == "mean" else 1.0
+        for got in (loss, only):
+            if reduction == "none":
+                assert torch.isnan(got[~good]).all()
+                close(got[good], want, tol)
+            else:
+                close(got, (want.sum() * f).reshape(1), (tol.sum() * f + ref.U * 2 * want.sum().abs() * f).reshape(1))
+        scale = 0.5 * f * weights[good].double()[:, None]
+        for got in (grad, again):
+            assert torch.isnan(got[~good]).all()
+            close(got[good], grad64 * scale,
+                  ref.grad_tolerance(grad64 * scale, x.dtype, vocab, scale * temperature, p, lp) + more * scale)
+
+
+# 8 blocks a row and one block a row for the step with the gradient; up to 480 entries and more
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(13, 50257), (160, 20011)])
+@pytest.mark.parametrize("top", [31, 64, 480, 481, 1024])
+def test_distillation_of_long_rows_duplicates_and_extremes(be, dtype, rows, vocab, top):
+    x = logits_for(rows, vocab, 0, dtype, top)
+    idx, val = teacher_for(rows, vocab, top, 11)
+    idx[0, -1] = idx[0, 0]                             # the same index first and last
+    idx[1, 3:27] = idx[1, 3].item()                    # many times in a row
+    idx[2] = vocab - 1                                 # all entries the same
+    val[3, 5:] = -math.inf                             # entries of no weight
+    val[4] = -math.inf                                 # no weight at all
+    val[5] = torch.finfo(torch.float32).min
+    idx[6, :-1] = -1                                   # only the last entry
+    idx[7, ::2] = idx[7, 1].item()
+    x[8] = torch.finfo(dtype).min                      # a uniform student
+    x[9, ::2] = -math.inf                              # masked, but not where the teacher looks
+    idx[9] = idx[9] | 1
+    check_special_distill(be, x, idx.clamp(max=vocab - 1), val, 1.0)
+    check_special_distill(be, x, idx.clamp(max=vocab - 1), val, 2.5)
+    x[10, idx[10, 0].long()] = -math.inf               # the student rules out what the teacher wants: infinite loss
+    x[11] = -math.inf                                  # or everything
+    check_special_distill(be, x, idx.clamp(max=vocab - 1), val, 1.0)
+    loss, _ = be.distillation_loss(x, idx.clamp(max=vocab - 1), val, reduction="none")
+    be.sync()
+    assert loss[4].item() == 0.0 and loss[10].item() == math.inf and loss[11].item() == math.inf
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(13, 50257), (160, 20011)])
+@pytest.mark.parametrize("top", [5, 100, 480, 481, 1024])
+def test_distillation_of_long_rows_nan_and_bad_indices(be, dtype, rows, vocab, top):
+    x = logits_for(rows, vocab, 0, dtype, top)
+    idx, val = teacher_for(rows, vocab, top, 12)
+    val[0, top - 1] = math.nan
+    val[1, 0] = math.inf
+    x[2, vocab - 1] = math.nan
+    x[3, vocab // 2] = math.inf
+    val[4] = math.nan
+    val[5, 1] = math.nan                               # of an entry that is missing: nobody looks at it
+    idx[5, 1] = -1
+    check_special_distill(be, x, idx, val, 1.0, nan_rows=(0, 1, 2, 3, 4))
+    for bad in (vocab, -2):
+        idx[6, top // 2] = bad
+        loss, grad = be.distillation_loss(x, idx, val, reduction="none")
+        with pytest.raises(IndexError):
+            be.sync()
+        idx[6, top // 2] = -1
+        same, same_grad = be.distillation_loss(x, idx, val, reduction="none")
+        be.sync()
+        assert torch.equal(loss[5:], same[5:]) and torch.equal(grad[5:], same_grad[5:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(1500, 515), (40, 6007), (13, 50257)])
+def test_score_gradient_where_the_token_is_an_alternative(be, dtype, rows, vocab):
+    """One index in the list twice: the gradients of both outputs meet in one place of the row."""
+    x = logits_for(rows, vocab, 0, dtype, 41)
+    check_score_grad(be, x, x.float().argmax(1), 1.0, 9)
+
+
+def test_captured_long_rows_replay_on_new_inputs(be):
+    """Calls whose rows are cut into clusters of blocks, and with shared memory that has to be asked for."""
+    x = logits_for(16, 50257, 0, torch.float32, 30)
+    tokens = torch.arange(16, device="cuda")
+    few, many = teacher_for(16, 50257, 64, 4), teacher_for(16, 50257, 700, 4)
+
+    def calls():
+        out = be.token_log_probs(x, tokens, top=200, entropy=True)
+        grad = be.token_log_probs_bwd(x, tokens, out.stats, d_log_probs=out.log_probs, entropy=out.entropy, d_entropy=out.entropy,
+                                      top_indices=out.top_indices, d_top=out.top_log_probs)
+        return list(out) + [grad] + list(be.distillation_loss(x, *few)) + list(be.distillation_loss(x, *many, reduction="none"))
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for round_ in range(3):
+        x.copy_(logits_for(16, 50257, 0, torch.float32, 50 + round_))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = calls()
+        be.sync()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_outputs_of_one_call_share_one_backward_pass(be, monkeypatch):
+    """Gradients of two and three outputs that meet in one scalar: the logits are gone through once."""
+    import minitensor_b200.nn as nn
+    from minitensor_b200.tensor import Tensor
+    passes = []
+    inner = be.token_log_probs_bwd
+    monkeypatch.setattr(be, "token_log_probs_bwd", lambda *a, **k: passes.append(sorted(n for n in k if k[n] is not None)) or inner(*a, **k))
+    rng = np.random.default_rng(1)
+    tokens = Tensor(rng.integers(0, 50, (3, 4)))
+    x = Tensor(rng.standard_normal((3, 4, 50)).astype(np.float32), requires_grad=True)
+    out = nn.token_log_probs(x, tokens, top=5, entropy=True)
+    (out.log_probs + out.entropy).sum().backward()
+    assert len(passes) == 1 and "d_log_probs" in passes[0] and "d_entropy" in passes[0] and "d_top" not in passes[0]
+    out = nn.token_log_probs(x, tokens, top=5, entropy=True)
+    (out.log_probs.sum() + out.entropy.sum() + out.top_log_probs.sum()).backward()
+    assert len(passes) == 2 and all(n in passes[1] for n in ("d_log_probs", "d_entropy", "d_top"))
+    out = nn.token_log_probs(x, tokens, top=5, entropy=True)
+    out.top_log_probs.sum().backward()
+    assert len(passes) == 3 and "d_top" in passes[2] and "d_log_probs" not in passes[2] and "d_entropy" not in passes[2]
