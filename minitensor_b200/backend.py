@@ -421,7 +421,7 @@ class Backend:
     def token_log_probs(self, logits: torch.Tensor, tokens: Optional[torch.Tensor], *, temperature: float = 1.0, top: int = 0,
                         entropy: bool = False, ignore_index: Optional[int] = None) -> TokenLogProbs:
         """Log probability of ``tokens[r]`` under ``softmax(logits[r] / temperature)``, the entropy of that distribution
-        and its ``top`` largest entries (best first, ties to the lower index), in one pass over ``logits``.
+        and its ``top`` largest entries (best first, ties to the lower index; 256 at most), in one pass over ``logits``.
 
         ``logits`` is ``[rows, vocabulary]`` in float32, float16 or bfloat16 with dense rows at any row stride;
         ``tokens`` ``[rows]`` int32 / int64 or ``None``.  Rows whose token is ``ignore_index`` are left out: 0, 0, and
@@ -506,7 +506,7 @@ class Backend:
                           stats: Optional[torch.Tensor] = None):
         """``temperature**2 * KL(q || softmax(logits / temperature))`` per row, where ``q`` is the softmax of
         ``teacher_logits / temperature`` over the teacher's entries ``[rows, entries]`` (logits or log probabilities;
-        index -1 marks a missing entry).  Returns ``(loss, dlogits or None)`` as :meth:`cross_entropy_ex` does; with
+        index -1 marks a missing entry; 1024 entries at most).  Returns ``(loss, dlogits or None)`` as :meth:`cross_entropy_ex` does; with
         ``stats`` (``[rows, 2]`` float32) the statistics for :meth:`distillation_loss_bwd` are kept there."""
         code, rows, vocab, ld, red, top = self._distill_checks("distillation_loss", logits, teacher_indices, teacher_logits,
                                                                reduction, upstream_rows, stats)

@@ -475,7 +475,7 @@ class TokenLogProbs(NamedTuple):
 def token_log_probs(input: Tensor, tokens: Tensor, temperature: float = 1.0, top: int = 0, entropy: bool = False,
                     ignore_index: Optional[int] = None) -> TokenLogProbs:
     """Log probability of one given token per position under ``softmax(input / temperature)``, with the entropy of that
-    distribution and its ``top`` most likely tokens on request (no counterpart in the reference).
+    distribution and its ``top`` most likely tokens (256 at most) on request (no counterpart in the reference).
 
     ``input`` holds float32 logits ``[..., vocabulary]``, ``tokens`` int32 / int64 indices ``[...]``.  Positions whose
     token is ``ignore_index`` are left out: 0, 0, alternatives of -inf with index -1, no gradient.  ``log_probs``,
@@ -528,11 +528,12 @@ def distillation_loss(input: Tensor, teacher_indices: Tensor, teacher_logits: Te
                       reduction: str = "mean") -> Tensor:
     """``temperature**2 * KL(q || softmax(input / temperature))`` where the teacher is known by its largest logits alone:
     ``q = softmax(teacher_logits / temperature)`` over the entries ``teacher_indices`` ``[..., entries]`` of each position,
-    index -1 marking a missing one (no counterpart in the reference).
+    1024 at most, index -1 marking a missing one (no counterpart in the reference).
 
     ``teacher_logits`` may be logits or log probabilities, e.g. the ``top_log_probs`` of :func:`token_log_probs` with its
     ``top_indices``; no gradient flows to them.  ``input`` holds float32 logits ``[..., vocabulary]``.  A position without
-    an entry has loss 0 and gradient 0; ``reduction`` "mean" divides by the number of positions."""
+    an entry has loss 0 and gradient 0; ``reduction`` "mean" divides by the number of positions, those without an entry
+    among them: over a padded batch take "sum" and divide by the number wanted."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"Invalid reduction mode: {reduction}. Must be 'mean', 'sum', or 'none'")
     if input.ndim < 1 or teacher_indices.ndim != input.ndim:
