@@ -3,6 +3,8 @@
 // counterpart in the reference; they stand beside its cross entropy (engine/src/operations/loss/regression.rs:178-251).
 // Every call is one or two launches, allocates nothing and keeps nothing between calls: statistics that a backward
 // call needs are the caller's.  Formulas, arithmetic and conventions: vocab_rows.cuh.
+// Times in the comments are of short runs of one call, at an SM clock of 1.965 GHz; under a sustained load the 1000 W cap leaves
+// 1.5 to 1.7 GHz, where calls with one exponential per 2 bytes or two per element take up to 20 % longer.
 #include "vocab_rows.cuh"
 
 #include <algorithm>
@@ -658,10 +660,15 @@ struct RowPlan {
 // A warp per row up to 8 KB where the rows are many (65536 x 1000 f32: 60 us against 460 us with a block of 512 per row; 300 x
 // 4000 f16 with 20 alternatives take 16.0 us by warps and 6.4 us by 128 threads, 2000 rows 20.8 and 15.7 us, 2000 x 1000 f32
 // 11.5 and 13.4 us), 128 threads up to 32 KB, or 64 KB with the selection, whose steps other rows have to hide (4096 x 16000
-// f32 with 20: 63 us against 100), else blocks of 512.  Many alternatives need many units to choose from: beyond WARP_TOP the warp, beyond MID_TOP the 128 threads are
-// the slower (8192 x 1000 f16 with 32: 99 us by warps and 64 us by blocks; 4096 x 4000 f32 with 100: 214 and 108 us).  Where
-// whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long as the parts still find room
-// side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us in 8, which run in two waves.
+// f32 with 20: 63 us against 100), else blocks of 512.  The number of rows is not looked at there: rows of 32 KB are at home with
+// 128 threads whether they are 1 or 2000 (16000 bf16 with 20: 7.1 us against 8.2, 24.9 against 31.1), those of 64 KB with the
+// selection only from some 500 on (32000 bf16 with 20, 128 threads against blocks of 512 in parts: 1 row 9.2 and 8.2 us, 300
+// rows 15.0 and 12.0, 600 rows 16.7 and 18.0, 2000 rows 36.9 and 42.6).
+// Many alternatives need many units to choose from: beyond WARP_TOP the warp, beyond MID_TOP the 128 threads are the slower
+// (8192 x 1000 f16 with 32: 99 us by warps and 64 us by blocks; 4096 x 4000 f32 with 100: 214 and 108 us).  Short rows with
+// more than MID_TOP are slow all the same: 4096 x 1000 f16 take 258 us with 128 and 46 with 64.
+// Where whole rows leave SMs without work, a row is cut into up to 8 parts of 8 KB at least, as long as the parts still find
+// room side by side: 64 rows of 128256 bf16 with their best 20 take 14.2 us in 4 parts and 24.7 us in 8, which run in two waves.
 constexpr int64_t WARP_BYTES = 8192, MID_BYTES = 32768, MID_BYTES_TOP = 65536, PART_BYTES = 8192;
 constexpr int WARP_TOP = 20, MID_TOP = 64;
 static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, bool warp, int64_t mid_bytes) {
@@ -673,9 +680,10 @@ static RowPlan plan_rows(const mtb200_ctx* h, int64_t rows, int64_t row_bytes, b
 }
 
 // With the selection on many rows, four blocks of 256 threads on an SM instead of two of 512: a block that selects leaves
-// three that stream.  4096 x 128256 bf16 and their best 20: 206 us against 239; 4096 x 60000 f32 180 against 213.  Rows that
-// take longer to stream gain nothing (2048 x 151936 f32 with 64: 247 us against 234), nor do fewer rows than blocks, and
-// from some 64 on the candidates are too many for 256 threads.
+// three that stream.  4096 x 128256 bf16 and their best 20: 206 us against 239; 4096 x 60000 f32 180 against 213.  Longer f32
+// rows, bound by HBM, gain nothing (2048 x 151936 with 64: 247 us against 234); of 16-bit ones, with twice the elements to
+// work on in a byte, all that were measured do (4096 x 151936 bf16 with 20: 232 us against 278, 1000 x 262144 f16: 102 against
+// 109).  Fewer rows than blocks gain nothing, and from some 64 on the candidates are too many for 256 threads.
 constexpr int64_t QUAD_BYTES = 256 << 10;
 template <typename T, int G>
 static int32_t launch_scores(mtb200_ctx* h, const ScoreArgs& a) {
@@ -723,7 +731,8 @@ static int32_t launch_score_grad(mtb200_ctx* h, const ScoreGradArgs& a) {
 }
 // Parts of a row for the step that looks at it twice: the rows in flight, three blocks of 512 threads on an SM, have to
 // stay in L2 beside the gradients that are written.  4096 x 128256 bf16, 114 MB of rows in flight without a cut: 435 us in 2
-// parts (57 MB), 518 in 1, 538 in 4, whose blocks do too little between their meetings.
+// parts (57 MB), 518 in 1, 538 in 4, whose blocks do too little between their meetings.  Parts are doubled: whether the rows
+// then fill whole waves of clusters is not looked at (1021 x 50257 f32 run as 4.6).
 constexpr int64_t L2_ROWS_BYTES = int64_t(64) << 20;
 template <typename T, int G>
 static int32_t launch_distill(mtb200_ctx* h, const DistillArgs& a) {
