@@ -506,8 +506,9 @@ class Backend:
                           stats: Optional[torch.Tensor] = None):
         """``temperature**2 * KL(q || softmax(logits / temperature))`` per row, where ``q`` is the softmax of
         ``teacher_logits / temperature`` over the teacher's entries ``[rows, entries]`` (logits or log probabilities;
-        index -1 marks a missing entry; 1024 entries at most).  Returns ``(loss, dlogits or None)`` as :meth:`cross_entropy_ex` does; with
-        ``stats`` (``[rows, 2]`` float32) the statistics for :meth:`distillation_loss_bwd` are kept there."""
+        index -1 marks a missing entry; 1024 entries at most).  Returns ``(loss, dlogits or None)`` as
+        :meth:`cross_entropy_ex` does; with ``stats`` (``[rows, 2]`` float32) the statistics for
+        :meth:`distillation_loss_bwd` are kept there."""
         code, rows, vocab, ld, red, top = self._distill_checks("distillation_loss", logits, teacher_indices, teacher_logits,
                                                                reduction, upstream_rows, stats)
         row_loss = torch.empty(rows, dtype=torch.float32, device=logits.device)

@@ -207,7 +207,9 @@ struct ScoreGradArgs {
 };
 
 // Blocks of a gradient kernel on an SM, which limit its registers: warps on 20000 x 1000 f32 with the entropy's gradient take 55 us
-// in four blocks and 63 in the three that fit without a limit, 20000 x 2000 bf16 without it 55 and 64.
+// in four blocks and 63 in the three that fit without a limit, 20000 x 2000 bf16 without it 55 and 64.  128 threads keep to the
+// eight or nine blocks that they just miss or just reach without one (4096 x 8000 f32: 59.5 us either way).  In 16 bits the
+// entropy's gradient needs 80 registers and more, and has them.
 template <typename T, int G, bool ENT>
 constexpr int grad_blocks() {
   return G == 512 ? 4 : sizeof(T) == 2 && ENT ? 1 : G == 32 ? 4 : sizeof(T) == 4 && !ENT ? 9 : 8;

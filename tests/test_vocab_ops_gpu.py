@@ -947,3 +947,41 @@ def test_outputs_of_one_call_share_one_backward_pass(be, monkeypatch):
     out = nn.token_log_probs(x, tokens, top=5, entropy=True)
     out.top_log_probs.sum().backward()
     assert len(passes) == 3 and "d_top" in passes[2] and "d_log_probs" not in passes[2] and "d_entropy" not in passes[2]
+
+
+def test_two_threads_with_a_backend_each(be):
+    """Handles share nothing but the record of granted shared memory: calls from two threads at once, on two streams."""
+    import threading
+    from minitensor_b200.backend import Backend
+    idx, val = teacher_for(16, 50257, 90, 5)
+    tokens = torch.arange(16, device="cuda")
+    xs = [logits_for(16, 50257, 0, torch.bfloat16, 70 + i) for i in range(2)]
+
+    def calls(b, x, top):
+        out = b.token_log_probs(x, tokens, top=top, entropy=True)
+        grad = b.token_log_probs_bwd(x, tokens, out.stats, d_log_probs=out.log_probs, top_indices=out.top_indices, d_top=out.top_log_probs)
+        return list(out) + [grad] + list(b.distillation_loss(x, idx, val))
+    want = [[calls(be, x, top) for top in range(100, 160, 3)] for x in xs]
+    be.sync()
+    others = [Backend(0) for _ in xs]
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = [calls(others[i], xs[i], top) for top in range(100, 160, 3)]
+                others[i].sync()
+        except Exception as e:  # reported below, in the test's own thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert all(torch.equal(p, q) for p, q in zip(a, b) if p is not None)
+    for b in others:
+        b.close()
